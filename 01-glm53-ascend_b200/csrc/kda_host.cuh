@@ -3,6 +3,9 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
+#include <mutex>
+
 namespace kda {
 
 inline int device_index() {
@@ -12,24 +15,34 @@ inline int device_index() {
 }
 
 inline int sm_count() {
-    static int count[64];
+    static std::atomic<int> count[64];
     const int dev = device_index();
-    if (count[dev] == 0) {
-        int c = 0;
+    int c = count[dev].load(std::memory_order_relaxed);
+    if (c == 0) {
         cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
-        count[dev] = c > 0 ? c : 1;
+        c = c > 0 ? c : 1;
+        count[dev].store(c, std::memory_order_relaxed);
     }
-    return count[dev];
+    return c;
 }
 
+// The dynamic shared memory that a kernel has been let have on each device.
+struct OptIn {
+    std::atomic<int> bytes[64];
+    std::mutex growing;
+};
+
 // Lets a kernel have `bytes` of dynamic shared memory; asked once per device
-// and growth (`done` is the kernel's own).
+// and growth (`done` is the kernel's own). Threads grow it in turn: the attribute
+// is the last value set, so a smaller one must never follow a larger one.
 template <typename K>
-inline bool opt_in(K kernel, int (&done)[64], int bytes) {
+inline bool opt_in(K kernel, OptIn &done, int bytes) {
     const int dev = device_index();
-    if (done[dev] >= bytes) return true;
+    if (done.bytes[dev].load(std::memory_order_acquire) >= bytes) return true;
+    const std::lock_guard<std::mutex> lock(done.growing);
+    if (done.bytes[dev].load(std::memory_order_relaxed) >= bytes) return true;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-    done[dev] = bytes;
+    done.bytes[dev].store(bytes, std::memory_order_release);
     return true;
 }
 

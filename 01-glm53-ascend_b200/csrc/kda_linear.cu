@@ -922,7 +922,7 @@ Choice choose(const KdaLinearArgs &a, int k_blocks) {
 
 template <typename O, bool E4M3, bool TMA_ROWS>
 cudaError_t launch_pair(const KdaLinearArgs &a, const Plan &plan, const Maps &maps, cudaStream_t st) {
-    static int opted[64];
+    static OptIn opted;
     if (!opt_in(pair_kernel<O, E4M3, TMA_ROWS>, opted, Pair::kBytes)) return cudaErrorInvalidValue;
     const int64_t tiles = static_cast<int64_t>(plan.tiles_t) * plan.tiles_n;
     const int pairs = static_cast<int>(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
@@ -932,7 +932,7 @@ cudaError_t launch_pair(const KdaLinearArgs &a, const Plan &plan, const Maps &ma
 template <typename O, bool E4M3, int BT, bool SEND>
 cudaError_t launch_narrow(const KdaLinearArgs &a, const Plan &plan, int splits, const Maps &maps, cudaStream_t st) {
     using C = Narrow<BT, SEND>;
-    static int opted[64];
+    static OptIn opted;
     if (!opt_in(narrow_kernel<O, E4M3, BT, SEND>, opted, C::kBytes)) return cudaErrorInvalidValue;
     const dim3 grid(static_cast<unsigned>(plan.tiles_n * splits), static_cast<unsigned>(plan.tiles_t));
     return launch_overlapped(narrow_kernel<O, E4M3, BT, SEND>, grid, C::kThreads, C::kBytes, splits, st, a, plan, splits, maps);

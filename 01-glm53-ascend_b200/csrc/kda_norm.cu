@@ -731,7 +731,7 @@ cudaError_t launch_rows(Rows rows, const KdaNormArgs &a, const Layout &l, cudaSt
 }
 template <typename T, bool FP8, bool RESIDUAL, int V>
 cudaError_t launch_ring_v(const KdaNormArgs &a, const RingLayout &r, cudaStream_t st) {
-    static int opted[64];
+    static OptIn opted;
     if (!opt_in(rmsnorm_ring_kernel<T, FP8, RESIDUAL, V>, opted, r.bytes)) return cudaErrorInvalidValue;
     return launch_overlapped(rmsnorm_ring_kernel<T, FP8, RESIDUAL, V>, dim3(r.grid), r.threads, r.bytes, 1, st, a, r.plan);
 }
@@ -766,7 +766,7 @@ cudaError_t launch(const KdaNormArgs &a, cudaStream_t st) {
 
 template <typename T, bool FP8, int D, int ACT, int V>
 cudaError_t launch_gated_ring(const KdaGatedNormArgs &a, const RingLayout &r, cudaStream_t st) {
-    static int opted[64];
+    static OptIn opted;
     if (!opt_in(gated_rmsnorm_ring_kernel<T, FP8, D, ACT, V>, opted, r.bytes)) return cudaErrorInvalidValue;
     return launch_overlapped(gated_rmsnorm_ring_kernel<T, FP8, D, ACT, V>, dim3(r.grid), r.threads, r.bytes, 1, st, a, r.plan);
 }

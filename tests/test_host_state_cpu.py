@@ -1,0 +1,75 @@
+"""Host state shared by the launchers' threads and devices (csrc/kda_host.cuh),
+compiled with a fake runtime: no GPU, no kernel."""
+
+import os
+import subprocess
+
+from conftest import PKG_DIR
+
+FAKE_RUNTIME = r"""
+#include <cuda_runtime.h>
+#include <atomic>
+#include <chrono>
+#include <cstdio>
+#include <thread>
+
+static thread_local int device = 0;
+static std::atomic<int> attribute[128];        // by device: the last value set
+static std::atomic<int> calls{0}, queries{0};
+static std::atomic<bool> hold_small{false}, large_set{false};
+
+static cudaError_t fake_get_device(int *dev) { return *dev = device, cudaSuccess; }
+static cudaError_t fake_get_attribute(int *v, cudaDeviceAttr, int dev) { return ++queries, *v = 100 + dev, cudaSuccess; }
+template <typename K>
+cudaError_t fake_set_attribute(K, cudaFuncAttribute, int bytes) {
+    ++calls;
+    // A thread that asks for little stands here until the larger request has gone through, or 300 ms.
+    for (int i = 0; hold_small && bytes < 1000 && !large_set && i < 300; ++i)
+        std::this_thread::sleep_for(std::chrono::milliseconds(1));
+    attribute[device] = bytes;
+    if (bytes >= 1000) large_set = true;
+    return cudaSuccess;
+}
+#define cudaGetDevice fake_get_device
+#define cudaDeviceGetAttribute fake_get_attribute
+#define cudaFuncSetAttribute fake_set_attribute
+#include "kda_host.cuh"
+#undef cudaGetDevice
+#undef cudaDeviceGetAttribute
+#undef cudaFuncSetAttribute
+
+static void kernel() {}
+// One kernel's opt-in, as a launcher holds it.
+static bool ask(int bytes) {
+    static kda::OptIn opted;
+    return kda::opt_in(&kernel, opted, bytes);
+}
+"""
+
+
+def run(tmp_path, body):
+    """The integers that a main() of `body` prints."""
+    src, exe = tmp_path / "host.cpp", tmp_path / "host"
+    src.write_text(FAKE_RUNTIME + "int main() {\n" + body + "\n}\n")
+    include = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", f"-I{include}", f"-I{PKG_DIR / 'csrc'}", str(src), "-o",
+                    str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True, timeout=60).stdout
+    return [int(v) for v in out.split()]
+
+
+def test_two_first_calls_leave_the_larger_opt_in(tmp_path):
+    """Two host threads whose first calls of one kernel need different sizes:
+    whichever is second, the kernel keeps the larger one."""
+    after, again, calls = run(tmp_path, r"""
+        hold_small = true;
+        std::thread small([] { ask(100); });
+        std::this_thread::sleep_for(std::chrono::milliseconds(50));   // inside its request by now
+        std::thread large([] { ask(2000); });
+        small.join(), large.join();
+        const int after = attribute[0];
+        const int before = calls;
+        ask(2000), ask(100), ask(1500);
+        printf("%d %d %d\n", after, attribute[0].load(), calls - before);
+    """)
+    assert after == 2000 and again == 2000 and calls == 0
