@@ -4,32 +4,38 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <map>
 #include <mutex>
 
 namespace kda {
 
-inline int device_index() {
+// What is remembered per device has a slot for each of the first 64 (-1: none).
+constexpr int kDeviceSlots = 64;
+
+inline int device_slot(int dev) { return dev >= 0 && dev < kDeviceSlots ? dev : -1; }
+
+inline int current_device() {
     int dev = 0;
-    cudaGetDevice(&dev);
-    return dev >= 0 && dev < 64 ? dev : 0;
+    return cudaGetDevice(&dev) == cudaSuccess ? dev : 0;
 }
 
 inline int sm_count() {
-    static std::atomic<int> count[64];
-    const int dev = device_index();
-    int c = count[dev].load(std::memory_order_relaxed);
+    static std::atomic<int> count[kDeviceSlots];
+    const int dev = current_device(), slot = device_slot(dev);
+    int c = slot >= 0 ? count[slot].load(std::memory_order_relaxed) : 0;
     if (c == 0) {
         cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
         c = c > 0 ? c : 1;
-        count[dev].store(c, std::memory_order_relaxed);
+        if (slot >= 0) count[slot].store(c, std::memory_order_relaxed);
     }
     return c;
 }
 
 // The dynamic shared memory that a kernel has been let have on each device.
 struct OptIn {
-    std::atomic<int> bytes[64];
+    std::atomic<int> bytes[kDeviceSlots];
     std::mutex growing;
+    std::map<int, int> beyond;   // devices without a slot
 };
 
 // Lets a kernel have `bytes` of dynamic shared memory; asked once per device
@@ -37,12 +43,15 @@ struct OptIn {
 // is the last value set, so a smaller one must never follow a larger one.
 template <typename K>
 inline bool opt_in(K kernel, OptIn &done, int bytes) {
-    const int dev = device_index();
-    if (done.bytes[dev].load(std::memory_order_acquire) >= bytes) return true;
+    const int dev = current_device(), slot = device_slot(dev);
+    if (slot >= 0 && done.bytes[slot].load(std::memory_order_acquire) >= bytes) return true;
     const std::lock_guard<std::mutex> lock(done.growing);
-    if (done.bytes[dev].load(std::memory_order_relaxed) >= bytes) return true;
+    if ((slot >= 0 ? done.bytes[slot].load(std::memory_order_relaxed) : done.beyond[dev]) >= bytes) return true;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-    done.bytes[dev].store(bytes, std::memory_order_release);
+    if (slot >= 0)
+        done.bytes[slot].store(bytes, std::memory_order_release);
+    else
+        done.beyond[dev] = bytes;
     return true;
 }
 

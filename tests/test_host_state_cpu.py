@@ -73,3 +73,19 @@ def test_two_first_calls_leave_the_larger_opt_in(tmp_path):
         printf("%d %d %d\n", after, attribute[0].load(), calls - before);
     """)
     assert after == 2000 and again == 2000 and calls == 0
+
+
+def test_devices_beyond_the_table(tmp_path):
+    """Device 70 takes neither device 0's opt-in nor its SM count, and keeps its own."""
+    got = run(tmp_path, r"""
+        const int sms = kda::sm_count();
+        ask(2000);
+        device = 70;
+        const int far = kda::sm_count();
+        ask(2000);
+        ask(100);
+        const int opted = attribute[70];
+        device = 0;
+        printf("%d %d %d %d %d\n", sms, far, opted, calls.load(), kda::sm_count());
+    """)
+    assert got == [100, 170, 2000, 2, 100]
