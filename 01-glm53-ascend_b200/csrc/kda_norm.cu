@@ -51,10 +51,13 @@ __device__ __forceinline__ Stats across_warps(Stats v, int warps, bool both, flo
 }
 
 // Eight neighbouring elements of a row as four pairs; one 16-byte access where the row allows it.
-template <typename T>
+// WRITTEN: the kernel may write over what it reads here (x and residual, which residual_out may
+// be), so the load must not take the read-only path.
+template <typename T, bool WRITTEN = false>
 __device__ __forceinline__ void load8(const T *p, bool aligned, float2 (&v)[4]) {
     if (aligned) {
-        const uint4 r = __ldg(reinterpret_cast<const uint4 *>(p));
+        const uint4 *at = reinterpret_cast<const uint4 *>(p);
+        const uint4 r = WRITTEN ? *at : __ldg(at);
         v[0] = unpack2<T>(r.x), v[1] = unpack2<T>(r.y), v[2] = unpack2<T>(r.z), v[3] = unpack2<T>(r.w);
     } else {
 #pragma unroll
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs 
         const int e = first(j);
         const bool whole = ROWS == ALIGNED ? e < columns : e >= 0 && e + 8 <= columns;
         if (whole) {
-            load8(x + e, true, v[j]);
+            load8<T, RESIDUAL>(x + e, true, v[j]);
         } else if (ROWS == SHIFTED && e < columns) {
             load8_part(x, e, columns, v[j]);
         } else {
@@ -171,7 +174,7 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs 
         }
         if (RESIDUAL && (whole || (ROWS == SHIFTED && e < columns))) {
             float2 r[4];
-            whole ? load8(res + e, true, r) : load8_part(res, e, columns, r);
+            whole ? load8<T, true>(res + e, true, r) : load8_part(res, e, columns, r);
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[j][k] = add2(v[j][k], r[k]);
         }
