@@ -18,6 +18,7 @@
 #include <type_traits>
 
 #include "kda_host.cuh"
+#include "kda_ring.cuh"
 #include "kda_rows.cuh"
 
 namespace kda {
@@ -506,6 +507,18 @@ __device__ __forceinline__ Ring ring_start(const RingPlan &plan, int inputs, uin
     return ring;
 }
 
+// A warp that does not meet a turn's copies leaves the loop, so that no stage is
+// filled or counted again whose copies have not landed; a block barrier goes on
+// without the warps that have left. What warp 0 had asked for gets one more wait
+// to land before the shared memory goes away (thread 0, having left at `turn`).
+template <typename First>
+__device__ __forceinline__ void ring_drain(const Ring &ring, int turn, int64_t rows, First first_row, int32_t *status) {
+    const RingTurns turns = {ring.plan.stages};
+    int32_t gave_up = 0;
+    for (const int end = turns.end_in_flight(turn); turn < end && first_row(turn) < rows; ++turn)
+        mbar_wait(&ring.full[turns.stage(turn)], turns.parity(turn), status, &gave_up);
+}
+
 // 80 registers let 24 warps of 4 vectors a thread be resident; with 16 at 104
 // registers the gated norm of 33,494 rows of 4,096 took 134 us against 125.
 constexpr int kRingRegisters = 80, kRingWarps = 24, kRingBytes = 200 * 1024, kMaxStages = 16;
@@ -524,10 +537,11 @@ __global__ void __maxnreg__(kRingRegisters) rmsnorm_ring_kernel(const KdaNormArg
     const Ring ring = ring_start(plan, RESIDUAL ? 2 : 1, full, &abort_word, fill);
     int stage = 0;
     uint32_t phase = 0;
-    for (int turn = 0; first_row(turn) < p.num_tokens; ++turn) {
+    int turn = 0;
+    for (; first_row(turn) < p.num_tokens; ++turn) {
         const int64_t row = first_row(turn) + sub;
         const bool live = row < p.num_tokens;
-        mbar_wait(&full[stage], phase, p.status, &abort_word);
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, p.status, &abort_word))) break;
         const uint8_t *x = ring.row(stage, sub, 0), *res = ring.row(stage, sub, RESIDUAL ? 1 : 0);
         float2 v[V][4], sum = make_float2(0.0f, 0.0f);
         float top = 0.0f;
@@ -580,8 +594,7 @@ __global__ void __maxnreg__(kRingRegisters) rmsnorm_ring_kernel(const KdaNormArg
                 store8(static_cast<T *>(p.out) + row * p.out_row_stride + i, true, v[j]);
         }
     }
-    // A wait ran out: one more gives the copies in flight the time to land.
-    if (abort_word != 0 && threadIdx.x == 0) mbar_wait(&full[stage], phase, p.status);
+    if (threadIdx.x == 0) ring_drain(ring, turn, p.num_tokens, first_row, p.status);
 }
 
 // What a turn adds to an address stays in registers here (64-bit products of
@@ -597,11 +610,12 @@ __global__ void __maxnreg__(kRingRegisters) gated_rmsnorm_ring_kernel(const KdaG
     const int threads = plan.warps * 32, tid = threadIdx.x % threads, sub = threadIdx.x / threads;
     const int vectors = p.num_heads * (D / 8);
     const int64_t step = static_cast<int64_t>(gridDim.x) * plan.rows;
+    const auto first_row = [&](int turn) { return turn * step + static_cast<int64_t>(blockIdx.x) * plan.rows; };
     const auto fill = [&](const Ring &ring, int stage, int turn) {
-        ring_fill(ring, stage, turn * step + static_cast<int64_t>(blockIdx.x) * plan.rows, p.num_tokens, static_cast<const uint8_t *>(p.o), p.o_stride[0] * 2,
+        ring_fill(ring, stage, first_row(turn), p.num_tokens, static_cast<const uint8_t *>(p.o), p.o_stride[0] * 2,
                   static_cast<const uint8_t *>(p.gate), p.gate_row_stride * 2);
     };
-    int64_t first = static_cast<int64_t>(blockIdx.x) * plan.rows;
+    int64_t first = first_row(0);
     const Ring ring = ring_start(plan, 2, full, &abort_word, fill);
     const int stage_bytes = plan.rows * 2 * plan.row_bytes, hop = threads * 8;
     const uint8_t *source = ring.row(0, sub, 0);
@@ -619,9 +633,10 @@ __global__ void __maxnreg__(kRingRegisters) gated_rmsnorm_ring_kernel(const KdaG
     }
     int stage = 0;
     uint32_t phase = 0;
-    for (int turn = 0; first < p.num_tokens; ++turn, first += step) {
+    int turn = 0;
+    for (; first < p.num_tokens; ++turn, first += step) {
         const bool live = first + sub < p.num_tokens;
-        mbar_wait(&full[stage], phase, p.status, &abort_word);
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, p.status, &abort_word))) break;
         const uint8_t *o = source + stage * stage_bytes, *gate = o + plan.row_bytes;
         float2 y[V][4];
         Stats st = {0.0f, 0.0f};
@@ -651,7 +666,7 @@ __global__ void __maxnreg__(kRingRegisters) gated_rmsnorm_ring_kernel(const KdaG
         }
         out += step * p.out_row_stride;
     }
-    if (abort_word != 0 && threadIdx.x == 0) mbar_wait(&full[stage], phase, p.status);
+    if (threadIdx.x == 0) ring_drain(ring, turn, p.num_tokens, first_row, p.status);
 }
 
 // How rows of `units` (vectors, or 8 single elements) are laid over a launch.

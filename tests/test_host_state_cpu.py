@@ -1,8 +1,11 @@
-"""Host state shared by the launchers' threads and devices (csrc/kda_host.cuh),
-compiled with a fake runtime: no GPU, no kernel."""
+"""What can be checked on the host of the norm and projection kernels: the
+launchers' state (csrc/kda_host.cuh) with a fake runtime, and the ring's
+bookkeeping (csrc/kda_ring.cuh). No GPU, no kernel."""
 
 import os
 import subprocess
+
+import pytest
 
 from conftest import PKG_DIR
 
@@ -47,10 +50,10 @@ static bool ask(int bytes) {
 """
 
 
-def run(tmp_path, body):
+def run(tmp_path, body, prelude=FAKE_RUNTIME):
     """The integers that a main() of `body` prints."""
     src, exe = tmp_path / "host.cpp", tmp_path / "host"
-    src.write_text(FAKE_RUNTIME + "int main() {\n" + body + "\n}\n")
+    src.write_text(prelude + "int main() {\n" + body + "\n}\n")
     include = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
     subprocess.run(["g++", "-std=c++17", "-O1", "-pthread", f"-I{include}", f"-I{PKG_DIR / 'csrc'}", str(src), "-o",
                     str(exe)], check=True)
@@ -89,3 +92,47 @@ def test_devices_beyond_the_table(tmp_path):
         printf("%d %d %d %d %d\n", sms, far, opted, calls.load(), kda::sm_count());
     """)
     assert got == [100, 170, 2000, 2, 100]
+
+
+RING = r"""
+#include <cstdio>
+#include <vector>
+#include "kda_ring.cuh"
+"""
+
+
+@pytest.mark.parametrize("stages", [2, 3, 6, 16])
+def test_ring_after_an_expired_wait(tmp_path, stages):
+    """Turn `stuck`'s copies do not land, as warp 0 of the norms' ring kernels goes
+    through its turns: no stage is filled twice without having been met, and what
+    is waited for at the end is all that is in flight, each on its own parity."""
+    got = run(tmp_path, r"""
+        int bad = 0, cases = 0;
+        for (int total = 1; total <= 40; ++total)
+            for (int stuck = 0; stuck <= total; ++stuck) {   // == total: nothing expires
+                const int stages = %d;
+                const kda::RingTurns turns = {stages};
+                std::vector<int> held(stages, -1), uses(stages, 0);   // the turn whose copies a stage waits for
+                const auto fill = [&](int turn) {
+                    if (turn >= total) return;                  // past the last row: nothing asked for
+                    bad += held[turn %% stages] >= 0;
+                    held[turn %% stages] = turn, ++uses[turn %% stages];
+                };
+                for (int i = 0; i < stages; ++i) fill(i);
+                int turn = 0;
+                for (; turn < total && turn != stuck; ++turn) {
+                    held[turn %% stages] = -1;                  // met
+                    fill(turn + stages);
+                }
+                std::vector<bool> waited(total, false);
+                for (const int end = turns.end_in_flight(turn); turn < end && turn < total; ++turn) {
+                    waited[turn] = true;
+                    bad += turns.stage(turn) != turn %% stages || held[turn %% stages] != turn;
+                    bad += static_cast<int>(turns.parity(turn)) != ((uses[turn %% stages] - 1) & 1);
+                }
+                for (int s = 0; s < stages; ++s) bad += held[s] >= 0 && !waited[held[s]];
+                ++cases;
+            }
+        printf("%%d %%d\n", bad, cases);
+    """ % stages, RING)
+    assert got == [0, 860]
