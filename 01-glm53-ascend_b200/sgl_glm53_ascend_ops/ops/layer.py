@@ -81,7 +81,8 @@ def _layer(step, hidden, w, residual, head_dim, **kwargs):
     T = hidden.shape[-2]
     H, R = w.A_log.numel(), w.decay_up.shape[1]
     C = 3 * H * head_dim
-    x = rmsnorm(hidden.reshape(T, -1), w.norm, None if residual is None else residual.reshape(T, -1), w.eps,
+    stream = hidden.reshape(T, hidden.shape[-1])   # T may be 0
+    x = rmsnorm(stream, w.norm, None if residual is None else residual.reshape(stream.shape), w.eps,
                 fp8=w.in_scale is not None)
     p = linear(x.out, w.in_proj, x_scale=x.scale, weight_scale=w.in_scale)
     a = linear(p[:, C:C + R], w.decay_up)
@@ -90,7 +91,8 @@ def _layer(step, hidden, w, residual, head_dim, **kwargs):
     o = step(mixed=p[:, :C], a=a, b=b, conv_weights=w.conv_weight, conv_bias=w.conv_bias, A_log=w.A_log,
              dt_bias=w.dt_bias, lower_bound=w.lower_bound, head_dim=head_dim, **kwargs)
     y = gated_rmsnorm(o[0], gate, w.out_norm, w.eps, fp8=w.out_scale is not None)
-    stream = hidden.reshape(T, -1) if residual is None else x.residual
+    if residual is not None:
+        stream = x.residual
     return linear(y.out, w.out_proj, residual=stream, x_scale=y.scale, weight_scale=w.out_scale).view(hidden.shape)
 
 
