@@ -329,7 +329,8 @@ __device__ __forceinline__ void gated8(const KdaGatedNormArgs &p, const float2 (
     for (int o = D / 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float rstd = rsqrtf(sum * (1.0f / D) + p.eps);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = mul2(mul2(y[e], make_float2(rstd, rstd)), mul2(w[e], activate2<ACT>(g[e])));
+    for (int e = 0; e < 4; ++e)   // from the left: w act(g) alone may pass fp32's range where y does not
+        y[e] = mul2(mul2(mul2(y[e], make_float2(rstd, rstd)), w[e]), activate2<ACT>(g[e]));
 }
 
 template <typename T, bool FP8, int D, int ACT, int V>
