@@ -503,13 +503,17 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) y[j] = make_float2(__uint_as_float(acc[2 * j]), __uint_as_float(acc[2 * j + 1]));
                 if (E4M3) {
+                    // The weight's scale, then the token's: their product alone may pass fp32's range. The token's by
+                    // single values, as pairs of it cost registers (8256 x 4096 outputs of K = 128: 19.6 us; by pairs,
+                    // spilled, 31).
+                    const auto scaled = [&](float2 v) { return make_float2(v.x * sx, v.y * sx); };
                     vector[lane] = h == 0 ? scale[0] : scale[1];
                     __syncwarp();
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float4 s = *reinterpret_cast<const float4 *>(vector + 4 * j);
-                        y[2 * j] = mul2(y[2 * j], mul2(make_float2(s.x, s.y), make_float2(sx, sx)));
-                        y[2 * j + 1] = mul2(y[2 * j + 1], mul2(make_float2(s.z, s.w), make_float2(sx, sx)));
+                        y[2 * j] = scaled(mul2(y[2 * j], make_float2(s.x, s.y)));
+                        y[2 * j + 1] = scaled(mul2(y[2 * j + 1], make_float2(s.z, s.w)));
                     }
                     __syncwarp();
                 }
@@ -754,8 +758,8 @@ __global__ void __launch_bounds__(Narrow<BT, SEND>::kThreads)
         }
         if (E4M3) {
             const float2 sx = make_float2(scales[r], scales[r]);
-            y[0] = mul2(y[0], mul2(make_float2(ws[0].x, ws[0].y), sx)), y[1] = mul2(y[1], mul2(make_float2(ws[0].z, ws[0].w), sx));
-            y[2] = mul2(y[2], mul2(make_float2(ws[1].x, ws[1].y), sx)), y[3] = mul2(y[3], mul2(make_float2(ws[1].z, ws[1].w), sx));
+            y[0] = mul2(mul2(y[0], make_float2(ws[0].x, ws[0].y)), sx), y[1] = mul2(mul2(y[1], make_float2(ws[0].z, ws[0].w)), sx);
+            y[2] = mul2(mul2(y[2], make_float2(ws[1].x, ws[1].y)), sx), y[3] = mul2(mul2(y[3], make_float2(ws[1].z, ws[1].w)), sx);
         }
         y[0] = add2(y[0], make_float2(bias[0].x, bias[0].y)), y[1] = add2(y[1], make_float2(bias[0].z, bias[0].w));
         y[2] = add2(y[2], make_float2(bias[1].x, bias[1].y)), y[3] = add2(y[3], make_float2(bias[1].z, bias[1].w));

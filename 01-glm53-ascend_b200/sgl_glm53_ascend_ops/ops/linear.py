@@ -24,7 +24,7 @@ def linear(
     activation: str = "none",
     out_dtype: Optional[torch.dtype] = None,
 ) -> torch.Tensor:
-    """``activation(x @ weight.T * x_scale[:, None] * weight_scale + bias) + residual``.
+    """``activation(x @ weight.T * weight_scale * x_scale[:, None] + bias) + residual``.
 
     x [T, K] or [1, T, K] and weight [N, K], both bf16, both fp16, or both
     float8_e4m3fn with fp32 scales per token and per output (see

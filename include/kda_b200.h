@@ -417,10 +417,10 @@ typedef struct KdaGatedNormArgs {
 int kda_gated_rmsnorm_launch(const KdaGatedNormArgs *args, void *stream);
 
 /* A projection with its epilogue:
- *   out[t, n] = round(act(x_scale[t] * weight_scale[n] * sum_k x[t, k] * weight[n, k] + bias[n]) + residual[t, n])
- * fp32 sums. x and weight are of one type: bf16 or fp16 (no scales), or e4m3
- * with both scales. out and residual are bf16 or fp16 (out_dtype; the type of
- * x when that is 16-bit). out may be residual itself, and overlaps no other input.
+ *   out[t, n] = round(act(x_scale[t] * (weight_scale[n] * sum_k x[t, k] * weight[n, k]) + bias[n]) + residual[t, n])
+ * fp32 sums, the scales multiplied in that order. x and weight are of one type:
+ * bf16 or fp16 (no scales), or e4m3 with both scales. out and residual are bf16
+ * or fp16 (out_dtype; the type of x when that is 16-bit). out may be residual itself, and overlaps no other input.
  * Operand rows that start on 16-byte boundaries with row strides that are
  * multiples of 16 bytes are read in place; others are first copied to such rows in the
  * workspace (kda_linear_workspace_bytes; 0 when nothing has to be copied). */
