@@ -51,6 +51,10 @@ __device__ __forceinline__ Stats across_warps(Stats v, int warps, bool both, flo
     return r;
 }
 
+template <typename T>
+__device__ __forceinline__ void unpack8(uint4 r, float2 (&v)[4]) {
+    v[0] = unpack2<T>(r.x), v[1] = unpack2<T>(r.y), v[2] = unpack2<T>(r.z), v[3] = unpack2<T>(r.w);
+}
 // Eight neighbouring elements of a row as four pairs; one 16-byte access where the row allows it.
 // WRITTEN: the kernel may write over what it reads here (x and residual, which residual_out may
 // be), so the load must not take the read-only path.
@@ -59,7 +63,7 @@ __device__ __forceinline__ void load8(const T *p, bool aligned, float2 (&v)[4]) 
     if (aligned) {
         const uint4 *at = reinterpret_cast<const uint4 *>(p);
         const uint4 r = WRITTEN ? *at : __ldg(at);
-        v[0] = unpack2<T>(r.x), v[1] = unpack2<T>(r.y), v[2] = unpack2<T>(r.z), v[3] = unpack2<T>(r.w);
+        unpack8<T>(r, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = make_float2(to_f32(p[2 * i]), to_f32(p[2 * i + 1]));
@@ -95,6 +99,19 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
+// The 8 weights from column e on, which are on 16 bytes.
+template <typename T>
+__device__ __forceinline__ void vector_weights(const KdaNormArgs &p, int e, float2 (&w)[4]) {
+    if (p.weight_fp32) {
+        const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + e);
+        const float4 a = __ldg(q), b = __ldg(q + 1);
+        w[0] = make_float2(a.x, a.y), w[1] = make_float2(a.z, a.w);
+        w[2] = make_float2(b.x, b.y), w[3] = make_float2(b.z, b.w);
+    } else {
+        load8(static_cast<const T *>(p.weight) + e, true, w);
+    }
+}
+
 // The scale of a row whose largest |y| is `top`; thread `lead` writes it. Returns its inverse.
 __device__ __forceinline__ float e4m3_inverse(float top, float *scale, int64_t row, bool lead) {
     const float s = max_nan(top * (1.0f / kE4m3Max), KDA_E4M3_SCALE_FLOOR);
@@ -128,10 +145,20 @@ __device__ __forceinline__ void store8_part(T *row, int e, int columns, const fl
     }
 }
 
+// The products s w for the e4m3 scale's maximum come ahead of the root. They are
+// held 2^32 times smaller: a row whose sum of squares is finite has |s| < 2^64, so
+// with weights below 2^96 none passes fp32's range unless y does, and a row
+// whose sum is infinite (root 0) gives zeros with weights below 2^32. What this takes
+// from the small end, |s w| < 2^-94, is far below the scale's floor for any eps
+// above 2^-112. A 16-bit output multiplies s by the root first, and loses nothing.
+constexpr float kDown = 0x1p-32f, kUp = 0x1p32f;
+
 // V units of 8 elements per thread: vectors, or (LOOSE) single elements
 // `threads` apart, which keeps a warp's 2-byte accesses side by side. The sum
-// with the residual is stored as soon as it is known; only s w is held until
-// the row's statistics have met.
+// with the residual is stored as soon as it is known; until the row's
+// statistics have met, s w is held for an e4m3 output, and s otherwise, with
+// the weights beside it where they are few (loaded afterwards they cost a row alone
+// their latency).
 template <typename T, bool FP8, bool RESIDUAL, Rows ROWS, int V>
 __global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs p, const int warps) {
     using Out = typename std::conditional<FP8, __nv_fp8_e4m3, T>::type;
@@ -180,57 +207,56 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs 
             for (int k = 0; k < 4; ++k) v[j][k] = add2(v[j][k], r[k]);
         }
     }
+    // The weights of unit j; zeros, or (SHIFTED) some weight, past the row's ends. ALIGNED units lie inside it.
+    const auto weights = [&](int j, float2 (&w)[4]) {
+        if constexpr (ROWS == ALIGNED) {
+            vector_weights<T>(p, first(j), w);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int a = ROWS == LOOSE ? loose(j, 2 * k) : first(j) + 2 * k, b = ROWS == LOOSE ? loose(j, 2 * k + 1) : a + 1;
+                if (ROWS == LOOSE)
+                    w[k] = make_float2(a < columns ? weight_at<T>(p.weight, p.weight_fp32, a) : 0.0f,
+                                       b < columns ? weight_at<T>(p.weight, p.weight_fp32, b) : 0.0f);
+                else
+                    w[k] = make_float2(weight_at<T>(p.weight, p.weight_fp32, min(max(a, 0), p.hidden - 1)),
+                                       weight_at<T>(p.weight, p.weight_fp32, min(max(b, 0), p.hidden - 1)));
+            }
+        }
+    };
+    constexpr bool kHeld = !FP8 && V <= 2;
+    float2 held[kHeld ? V : 1][4];
     float top = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        float2 w[4];
-        if (ROWS == LOOSE) {
+        if (ROWS == ALIGNED && first(j) >= columns) continue;
+        if (RESIDUAL && p.residual_out != nullptr) {
+            if (ROWS == LOOSE) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int a = loose(j, 2 * k), b = loose(j, 2 * k + 1);
-                w[k] = make_float2(a < columns ? weight_at<T>(p.weight, p.weight_fp32, a) : 0.0f,
-                                   b < columns ? weight_at<T>(p.weight, p.weight_fp32, b) : 0.0f);
-                if (RESIDUAL && p.residual_out != nullptr) {
+                for (int k = 0; k < 4; ++k) {
+                    const int a = loose(j, 2 * k), b = loose(j, 2 * k + 1);
                     if (a < columns) res_out[a] = from_f32<T>(v[j][k].x);
                     if (b < columns) res_out[b] = from_f32<T>(v[j][k].y);
                 }
-            }
-        } else {
-            const int e = first(j);
-            const bool whole = ROWS == ALIGNED ? e < columns : e >= 0 && e + 8 <= columns;
-            if (RESIDUAL && p.residual_out != nullptr) {
-                if (whole)
+            } else {
+                const int e = first(j);
+                if (ROWS == ALIGNED || (e >= 0 && e + 8 <= columns))
                     store8(res_out + e, true, v[j]);
-                else if (ROWS == SHIFTED)
+                else
                     store8_part(res_out, e, columns, v[j]);
             }
-            if (ROWS == SHIFTED) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int a = min(max(e + 2 * k, 0), p.hidden - 1), b = min(max(e + 2 * k + 1, 0), p.hidden - 1);
-                    w[k] = make_float2(weight_at<T>(p.weight, p.weight_fp32, a), weight_at<T>(p.weight, p.weight_fp32, b));
-                }
-            } else if (whole && p.weight_fp32) {
-                const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + e);
-                const float4 a = __ldg(q), b = __ldg(q + 1);
-                w[0] = make_float2(a.x, a.y), w[1] = make_float2(a.z, a.w);
-                w[2] = make_float2(b.x, b.y), w[3] = make_float2(b.z, b.w);
-            } else if (whole) {
-                load8(static_cast<const T *>(p.weight) + e, true, w);
-            } else {
-                continue;
-            }
         }
+        float2 w[4];
+        if (FP8) weights(j, w);
+        if (kHeld) weights(j, held[j]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             sum = fma2(v[j][k], v[j][k], sum);
-            if (ROWS == SHIFTED) {
-                // Past the ends v is zero, and a weight of infinity or NaN must not reach the maximum.
+            if (!FP8) continue;
+            v[j][k] = make_float2(v[j][k].x * kDown * w[k].x, v[j][k].y * kDown * w[k].y);   // singly: pairs spill
+            if (ROWS == SHIFTED) {   // a weight of infinity or NaN must not reach the maximum from past the ends
                 const int a = first(j) + 2 * k;
-                v[j][k] = make_float2(a >= 0 && a < columns ? v[j][k].x * w[k].x : 0.0f,
-                                      a + 1 >= 0 && a + 1 < columns ? v[j][k].y * w[k].y : 0.0f);
-            } else {
-                v[j][k] = mul2(v[j][k], w[k]);
+                v[j][k] = make_float2(a >= 0 && a < columns ? v[j][k].x : 0.0f, a + 1 >= 0 && a + 1 < columns ? v[j][k].y : 0.0f);
             }
         }
         if (FP8) top = max8(top, v[j]);
@@ -239,11 +265,21 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs 
     if (warps > 1) st = across_warps(st, warps, true, part);
     if (!live) return;
     float m = rsqrtf(st.sum / p.hidden + p.eps);
-    if (FP8) m *= e4m3_inverse(st.top * m, p.scale, row, tid == 0);
+    if (FP8) {
+        m *= kUp;
+        m *= e4m3_inverse(st.top * m, p.scale, row, tid == 0);
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[j][k] = mul2(v[j][k], make_float2(m, m));
+        if (ROWS == ALIGNED && first(j) >= columns) continue;
+        if (!FP8) {
+            float2 w[4];
+            if (!kHeld) weights(j, w);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j][k] = mul2(v[j][k], kHeld ? held[j][k] : w[k]);
+        }
         if (ROWS == LOOSE) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -254,9 +290,9 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs 
             continue;
         }
         const int e = first(j);
-        if (ROWS == ALIGNED ? e < columns : e >= 0 && e + 8 <= columns)
+        if (ROWS == ALIGNED || (e >= 0 && e + 8 <= columns))
             store8(out + e, true, v[j]);
-        else if (ROWS == SHIFTED)
+        else
             store8_part(out, e, columns, v[j]);
     }
 }
@@ -276,19 +312,18 @@ __global__ void __launch_bounds__(kLongThreads) rmsnorm_long_kernel(const KdaNor
         float s = to_f32(x[i]);
         if (res != nullptr) s += to_f32(res[i]);
         st.sum = fmaf(s, s, st.sum);
-        if (FP8) st.top = max_nan(st.top, fabsf(s * weight_at<T>(p.weight, p.weight_fp32, i)));
+        if (FP8) st.top = max_nan(st.top, fabsf(s * kDown * weight_at<T>(p.weight, p.weight_fp32, i)));
     }
     st = {warp_sum(st.sum), warp_max_nan(st.top)};
     st = across_warps(st, kLongThreads / 32, true, part);
     const float rstd = rsqrtf(st.sum / p.hidden + p.eps);
-    float m = rstd;
-    if (FP8) m *= e4m3_inverse(st.top * rstd, p.scale, row, threadIdx.x == 0);
+    const float inv = FP8 ? e4m3_inverse(st.top * (rstd * kUp), p.scale, row, threadIdx.x == 0) : 1.0f;
     for (int64_t i = threadIdx.x; i < p.hidden; i += kLongThreads) {
         float s = to_f32(x[i]);
         if (res != nullptr) s += to_f32(res[i]);
-        const float y = s * m * weight_at<T>(p.weight, p.weight_fp32, i);
+        const float y = s * rstd * weight_at<T>(p.weight, p.weight_fp32, i);
         if (FP8)
-            static_cast<__nv_fp8_e4m3 *>(p.out)[row * p.out_row_stride + i] = from_f32<__nv_fp8_e4m3>(y);
+            static_cast<__nv_fp8_e4m3 *>(p.out)[row * p.out_row_stride + i] = from_f32<__nv_fp8_e4m3>(y * inv);
         else
             static_cast<T *>(p.out)[row * p.out_row_stride + i] = from_f32<T>(y);
         if (rout != nullptr) rout[i] = from_f32<T>(s);
@@ -450,8 +485,7 @@ __device__ __forceinline__ void ring_fill(const Ring &ring, int stage, int64_t f
 
 template <typename T>
 __device__ __forceinline__ void load8_shared(const uint8_t *p, float2 (&v)[4]) {
-    const uint4 r = *reinterpret_cast<const uint4 *>(p);
-    v[0] = unpack2<T>(r.x), v[1] = unpack2<T>(r.y), v[2] = unpack2<T>(r.z), v[3] = unpack2<T>(r.w);
+    unpack8<T>(*reinterpret_cast<const uint4 *>(p), v);
 }
 
 // What the warps of a CTA tell one another, double-buffered by turn so that
@@ -545,6 +579,9 @@ __global__ void __maxnreg__(kRingRegisters) rmsnorm_ring_kernel(const KdaNormArg
         if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, p.status, &abort_word))) break;
         const uint8_t *x = ring.row(stage, sub, 0), *res = ring.row(stage, sub, RESIDUAL ? 1 : 0);
         float2 v[V][4], sum = make_float2(0.0f, 0.0f);
+        // A 16-bit output's first weights, ahead of the exchange; the others come after it. 33,494 rows of 4,096 with
+        // residual 176 us, 8,000 of 8,192 86; none ahead 177 and 90; two, packed, 186 and 90.
+        float2 ahead[4];
         float top = 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -559,36 +596,40 @@ __global__ void __maxnreg__(kRingRegisters) rmsnorm_ring_kernel(const KdaNormArg
                     if (p.residual_out != nullptr)
                         store8(static_cast<T *>(p.residual_out) + row * p.residual_out_row_stride + i, true, v[j]);
                 }
-                float2 w[4];
-                if (p.weight_fp32) {
-                    const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + i);
-                    const float4 a = __ldg(q), b = __ldg(q + 1);
-                    w[0] = make_float2(a.x, a.y), w[1] = make_float2(a.z, a.w);
-                    w[2] = make_float2(b.x, b.y), w[3] = make_float2(b.z, b.w);
-                } else {
-                    load8(static_cast<const T *>(p.weight) + i, true, w);
-                }
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    sum = fma2(v[j][e], v[j][e], sum);
-                    v[j][e] = mul2(v[j][e], w[e]);
+                for (int e = 0; e < 4; ++e) sum = fma2(v[j][e], v[j][e], sum);
+                if (FP8) {
+                    float2 w[4];
+                    vector_weights<T>(p, i, w);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[j][e] = mul2(mul2(v[j][e], make_float2(kDown, kDown)), w[e]);
+                    top = max8(top, v[j]);
                 }
-                if (FP8) top = max8(top, v[j]);
             }
         }
+        if (!FP8 && tid * 8 < p.hidden) vector_weights<T>(p, tid * 8, ahead);
         Stats st = {warp_sum(sum.x + sum.y), FP8 ? warp_max_nan(top) : 0.0f};
         st = ring_exchange<true, FP8>(st, plan.warps, part, turn & 1);
         if (threadIdx.x < 32) fill(ring, stage, turn + plan.stages);
         if (++stage == plan.stages) stage = 0, phase ^= 1;
         if (!live) continue;
         float m = rsqrtf(st.sum / p.hidden + p.eps);
-        if (FP8) m *= e4m3_inverse(st.top * m, p.scale, row, tid == 0);
+        if (FP8) {
+            m *= kUp;
+            m *= e4m3_inverse(st.top * m, p.scale, row, tid == 0);
+        }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int i = (j * threads + tid) * 8;
             if (i >= p.hidden) continue;
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[j][e] = mul2(v[j][e], make_float2(m, m));
+            if (!FP8) {
+                float2 w[4];
+                if (j > 0) vector_weights<T>(p, i, w);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[j][e] = mul2(v[j][e], j > 0 ? w[e] : ahead[e]);
+            }
             if (FP8)
                 store8(static_cast<__nv_fp8_e4m3 *>(p.out) + row * p.out_row_stride + i, true, v[j]);
             else

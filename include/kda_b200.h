@@ -365,8 +365,9 @@ typedef enum KdaActivation {
  *   y = s / sqrt(mean(s^2) + eps) * weight
  *   out = round(y), or, when scale is given, for each row
  *   scale = max(max|y| / 448, KDA_E4M3_SCALE_FLOOR), out = e4m3(y * (1 / scale)).
- * Statistics are fp32 sums over the unrounded s, so a row whose sum of squares
- * passes fp32's range (3.4e38) comes out as zeros. A NaN or infinity spreads
+ * Statistics are fp32 sums over the unrounded s, so a finite row whose sum of
+ * squares passes fp32's range (3.4e38) comes out as zeros (with a scale, for
+ * weights below 2^32). A NaN or infinity spreads
  * over its own row (its scale included) and to no other row. residual_out may
  * be residual or x itself. Rows may start anywhere: 16-byte vectors are used
  * where every pointer and row stride allows them. */
