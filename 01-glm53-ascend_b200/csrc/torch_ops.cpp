@@ -555,6 +555,9 @@ at::Tensor empty_like_type(const at::Tensor &t, at::IntArrayRef sizes, at::Scala
     return at::detail::empty_cuda(sizes, type, t.device(), c10::nullopt);
 }
 
+// An optional result: none where it was not made.
+c10::optional<at::Tensor> given(const at::Tensor &t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; }
+
 int32_t kda_dtype(const char *op, const char *name, const at::Tensor &t, bool e4m3 = false) {
     if (t.scalar_type() == at::kBFloat16) return KDA_DTYPE_BF16;
     if (t.scalar_type() == at::kHalf) return KDA_DTYPE_FP16;
@@ -598,9 +601,8 @@ bool check_norm_weight(const char *op, const at::Tensor &weight, const at::Tenso
 //   residual  shape and type of x, or None
 //   fp8       e4m3 output with one fp32 scale per token
 // Returns (out, scale [T] or None, x + residual or None).
-std::tuple<at::Tensor, at::Tensor, at::Tensor> kda_rmsnorm(const at::Tensor &x, const at::Tensor &weight,
-                                                           const c10::optional<at::Tensor> &residual, double eps,
-                                                           bool fp8) {
+std::tuple<at::Tensor, c10::optional<at::Tensor>, c10::optional<at::Tensor>> kda_rmsnorm(
+    const at::Tensor &x, const at::Tensor &weight, const c10::optional<at::Tensor> &residual, double eps, bool fp8) {
     const char *op = "kda_rmsnorm";
     TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor");
     KdaNormArgs a{};
@@ -637,7 +639,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> kda_rmsnorm(const at::Tensor &x, 
     a.eps = static_cast<float>(eps);
     a.status = status_ptr(x.device());
     if (T > 0) check_kda(kda_rmsnorm_launch(&a, current_stream(x)), op);
-    return {out, scale, residual_out};
+    return {out, given(scale), given(residual_out)};
 }
 
 // kda_gated_rmsnorm: the per-head norm of the KDA output times act(gate)
@@ -646,9 +648,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> kda_rmsnorm(const at::Tensor &x, 
 //   gate    the same shape, or [T, H * D] / [1, T, H * D]; type of o
 //   weight  [D] fp32 or the type of o
 // Returns (out [T, H * D] or [1, T, H * D], scale [T] or None).
-std::tuple<at::Tensor, at::Tensor> kda_gated_rmsnorm(const at::Tensor &o, const at::Tensor &gate,
-                                                     const at::Tensor &weight, double eps,
-                                                     c10::string_view activation, bool fp8) {
+std::tuple<at::Tensor, c10::optional<at::Tensor>> kda_gated_rmsnorm(const at::Tensor &o, const at::Tensor &gate,
+                                                                    const at::Tensor &weight, double eps,
+                                                                    c10::string_view activation, bool fp8) {
     const char *op = "kda_gated_rmsnorm";
     TORCH_CHECK(o.is_cuda(), "o must be a CUDA tensor");
     KdaGatedNormArgs a{};
@@ -698,7 +700,7 @@ std::tuple<at::Tensor, at::Tensor> kda_gated_rmsnorm(const at::Tensor &o, const 
     a.eps = static_cast<float>(eps);
     a.status = status_ptr(o.device());
     if (T > 0) check_kda(kda_gated_rmsnorm_launch(&a, current_stream(o)), op);
-    return {out, scale};
+    return {out, given(scale)};
 }
 
 // kda_linear: a projection with its epilogue (kda_linear_launch):
@@ -820,9 +822,9 @@ TORCH_LIBRARY(sgl_glm53_ascend, m) {
           "Tensor query_start_loc, Tensor? has_initial_state=None, Tensor? track_conv_indices=None, "
           "Tensor? track_conv_lens=None, int num_parts=3, bool silu=True) -> Tensor");
     m.def("kda_rmsnorm(Tensor x, Tensor weight, Tensor? residual=None, float eps=1e-06, bool fp8=False) -> "
-          "(Tensor, Tensor, Tensor)");
+          "(Tensor, Tensor?, Tensor?)");
     m.def("kda_gated_rmsnorm(Tensor o, Tensor gate, Tensor weight, float eps=1e-06, str activation='sigmoid', "
-          "bool fp8=False) -> (Tensor, Tensor)");
+          "bool fp8=False) -> (Tensor, Tensor?)");
     m.def("kda_linear(Tensor x, Tensor weight, Tensor? bias=None, Tensor? residual=None, Tensor? x_scale=None, "
           "Tensor? weight_scale=None, str activation='none', ScalarType? out_dtype=None) -> Tensor");
     m.def("kda_set_status_buffer(int device, Tensor? buf) -> ()");

@@ -136,3 +136,13 @@ def test_ring_after_an_expired_wait(tmp_path, stages):
         printf("%%d %%d\n", bad, cases);
     """ % stages, RING)
     assert got == [0, 860]
+
+
+def test_schemas_say_which_results_may_be_none():
+    """scale without an e4m3 output, the sum without a residual."""
+    import torch
+    import sgl_glm53_ascend_ops  # noqa: F401
+
+    ns = torch.ops.sgl_glm53_ascend
+    assert str(ns.kda_rmsnorm.default._schema).endswith("bool fp8=False) -> (Tensor, Tensor?, Tensor?)")
+    assert str(ns.kda_gated_rmsnorm.default._schema).endswith("bool fp8=False) -> (Tensor, Tensor?)")
