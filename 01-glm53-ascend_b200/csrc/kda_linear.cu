@@ -903,6 +903,7 @@ struct Choice {
 // 23.9; 512 tokens, N = 4096 bf16: 128 (64 tiles) 21.7, 256 (32) 27.0.
 Choice choose(const KdaLinearArgs &a, int k_blocks) {
     const int64_t T = a.num_tokens, outputs = (static_cast<int64_t>(a.out_features) + kLanes - 1) / kLanes, sms = sm_count();
+    const int64_t pairs = sms > 1 ? sms / 2 : 1;
     for (int tile = 16; tile <= 64; tile *= 2) {
         const int64_t ctas = outputs * ((T + tile - 1) / tile);
         if (ctas > sms && (T > 64 || tile < T)) continue;
@@ -918,7 +919,7 @@ Choice choose(const KdaLinearArgs &a, int k_blocks) {
         const int width = 64 * (i + 1);
         const int64_t tiles = (T + Pair::kTileT - 1) / Pair::kTileT * ((a.out_features + width - 1) / width);
         const int64_t products = static_cast<int64_t>(k_blocks) * kBlockCycles[i], epilogue = 2600 + 6 * width;
-        const int64_t cycles = (tiles + sms / 2 - 1) / (sms / 2) * (products > epilogue ? products : epilogue);
+        const int64_t cycles = (tiles + pairs - 1) / pairs * (products > epilogue ? products : epilogue);
         if (cycles < least) least = cycles, best.tile = width;
     }
     return best;
@@ -929,7 +930,7 @@ cudaError_t launch_pair(const KdaLinearArgs &a, const Plan &plan, const Maps &ma
     static OptIn opted;
     if (!opt_in(pair_kernel<O, E4M3, TMA_ROWS>, opted, Pair::kBytes)) return cudaErrorInvalidValue;
     const int64_t tiles = static_cast<int64_t>(plan.tiles_t) * plan.tiles_n;
-    const int pairs = static_cast<int>(tiles < sm_count() / 2 ? tiles : sm_count() / 2);
+    const int most = sm_count() > 1 ? sm_count() / 2 : 1, pairs = static_cast<int>(tiles < most ? tiles : most);
     return launch_overlapped(pair_kernel<O, E4M3, TMA_ROWS>, dim3(2 * pairs), Pair::kThreads, Pair::kBytes, 2, st, a, plan, maps);
 }
 
