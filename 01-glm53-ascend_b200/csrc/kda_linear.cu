@@ -883,13 +883,6 @@ bool encode(CUtensorMap *map, const void *base, int32_t dtype, int64_t rows, int
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Which kernel, its tile and its splits.
-struct Choice {
-    bool pair;
-    int tile;      // outputs of the pair kernel's tile, tokens of the narrow one's
-    int splits;
-};
-
 // Few tokens: the narrow kernel with the smallest token tile whose tiles fit
 // one per SM, then K split until two CTAs per SM are busy (each with 4 blocks
 // of K at least). Measured, us (bf16, K = 4096; tile/splits): 64 tokens, N =
@@ -901,8 +894,8 @@ struct Choice {
 // cycles at widths 64..256) or its epilogue, whichever is longer. 256 tokens,
 // N = 12576, K = 4096 e4m3: width 192 (66 tiles) 17.7 us, 256 (50) 19.3, 128 (99)
 // 23.9; 512 tokens, N = 4096 bf16: 128 (64 tiles) 21.7, 256 (32) 27.0.
-Choice choose(const KdaLinearArgs &a, int k_blocks) {
-    const int64_t T = a.num_tokens, outputs = (static_cast<int64_t>(a.out_features) + kLanes - 1) / kLanes, sms = sm_count();
+KdaLinearForm choose(const KdaLinearArgs &a, int64_t k_blocks, int64_t sms) {
+    const int64_t T = a.num_tokens, outputs = (static_cast<int64_t>(a.out_features) + kLanes - 1) / kLanes;
     const int64_t pairs = sms > 1 ? sms / 2 : 1;
     for (int tile = 16; tile <= 64; tile *= 2) {
         const int64_t ctas = outputs * ((T + tile - 1) / tile);
@@ -910,19 +903,30 @@ Choice choose(const KdaLinearArgs &a, int k_blocks) {
         int64_t splits = 2 * sms / ctas;
         if (splits > k_blocks / 4) splits = k_blocks / 4;
         if (splits > 8) splits = 8;
-        return {false, tile, splits > 1 ? static_cast<int>(splits) : 1};
+        return {KDA_LINEAR_NARROW, tile, splits > 1 ? static_cast<int32_t>(splits) : 1};
     }
     static constexpr int kBlockCycles[4] = {345, 345, 425, 525};
-    Choice best = {true, 256, 1};
+    KdaLinearForm best = {KDA_LINEAR_PAIR, 256, 1};
     int64_t least = INT64_MAX;
     for (int i = 3; i >= 0; --i) {
         const int width = 64 * (i + 1);
         const int64_t tiles = (T + Pair::kTileT - 1) / Pair::kTileT * ((a.out_features + width - 1) / width);
-        const int64_t products = static_cast<int64_t>(k_blocks) * kBlockCycles[i], epilogue = 2600 + 6 * width;
+        const int64_t products = k_blocks * kBlockCycles[i], epilogue = 2600 + 6 * width;
         const int64_t cycles = (tiles + pairs - 1) / pairs * (products > epilogue ? products : epilogue);
         if (cycles < least) least = cycles, best.tile = width;
     }
     return best;
+}
+
+int k_blocks_of(const KdaLinearArgs &a) {
+    const int per = kRowBytes / element_bytes(a.in_dtype);
+    return (a.in_features + per - 1) / per;
+}
+// Whether any arguments of `k_blocks` may be launched in this form.
+bool form_ok(const KdaLinearArgs &a, int k_blocks, const KdaLinearForm &f) {
+    if (f.kernel == KDA_LINEAR_PAIR) return f.splits == 1 && f.tile >= 64 && f.tile <= Pair::kMaxN && f.tile % 64 == 0;
+    return f.kernel == KDA_LINEAR_NARROW && (f.tile == 16 || f.tile == 32 || f.tile == 64) && f.splits >= 1 && f.splits <= 8 &&
+           f.splits <= k_blocks && (a.num_tokens + f.tile - 1) / f.tile <= 65535;   // the grid's second dimension
 }
 
 template <typename O, bool E4M3, bool TMA_ROWS>
@@ -944,13 +948,14 @@ cudaError_t launch_narrow(const KdaLinearArgs &a, const Plan &plan, int splits, 
 }
 
 template <typename O, bool E4M3>
-cudaError_t launch_choice(const KdaLinearArgs &a, Plan plan, const Choice &c, const Maps &maps, cudaStream_t st) {
+cudaError_t launch_form(const KdaLinearArgs &a, Plan plan, const KdaLinearForm &c, const Maps &maps, cudaStream_t st) {
     const uint32_t format = a.in_dtype == KDA_DTYPE_BF16 ? 1 : 0;
-    plan.idesc = c.pair ? instruction_desc(256, c.tile, format) : instruction_desc(kLanes, c.tile, format);
+    const bool pair = c.kernel == KDA_LINEAR_PAIR;
+    plan.idesc = pair ? instruction_desc(256, c.tile, format) : instruction_desc(kLanes, c.tile, format);
     plan.width = c.tile;
     plan.tail = (a.out_features - (plan.tiles_n - 1) * c.tile + 31) / 32 * 32;
     plan.idesc_tail = instruction_desc(256, plan.tail, format);
-    if (c.pair) {
+    if (pair) {
         const bool tma_rows = plan.out_tma && (a.residual == nullptr || plan.residual_tma);
         return tma_rows ? launch_pair<O, E4M3, true>(a, plan, maps, st) : launch_pair<O, E4M3, false>(a, plan, maps, st);
     }
@@ -985,23 +990,19 @@ int check(const KdaLinearArgs *args) {
     return KDA_OK;
 }
 
-}  // namespace linear
-}  // namespace kda
-
-extern "C" size_t kda_linear_workspace_bytes(const KdaLinearArgs *args) {
-    using namespace kda::linear;
-    if (check(args) != KDA_OK || args->num_tokens == 0 || args->out_features == 0) return 0;
-    return (copies_x(*args) ? copy_bytes(*args, args->num_tokens) : 0) +
-           (copies_weight(*args) ? copy_bytes(*args, args->out_features) : 0);
+size_t workspace_bytes_of(const KdaLinearArgs &a) {
+    return (copies_x(a) ? copy_bytes(a, a.num_tokens) : 0) + (copies_weight(a) ? copy_bytes(a, a.out_features) : 0);
 }
 
-extern "C" int kda_linear_launch(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes, void *stream) {
-    using namespace kda::linear;
+// In the form given, or the one that choose() takes where it is null.
+int launch(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes, const KdaLinearForm *form, cudaStream_t st) {
     const int rc = check(args);
     if (rc != KDA_OK || args->num_tokens == 0 || args->out_features == 0) return rc;
     KdaLinearArgs a = *args;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const size_t need = kda_linear_workspace_bytes(args);
+    const int k_blocks = k_blocks_of(a);
+    const KdaLinearForm c = form != nullptr ? *form : choose(a, k_blocks, sm_count());
+    if (!form_ok(a, k_blocks, c)) return KDA_ERR_INVALID_ARGUMENT;
+    const size_t need = workspace_bytes_of(*args);
     if (need > 0) {
         if (workspace == nullptr || workspace_bytes < need) return KDA_ERR_WORKSPACE;
         if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return KDA_ERR_ALIGNMENT;
@@ -1024,15 +1025,15 @@ extern "C" int kda_linear_launch(const KdaLinearArgs *args, void *workspace, siz
         const int threads = kCopyWarps * 32;
         const cudaError_t e =
             a.in_dtype == KDA_DTYPE_E4M3
-                ? kda::launch_overlapped(realign_kernel<uint8_t>, grid, threads, 0, 1, st, copies[0], copies[1], a.in_features)
-                : kda::launch_overlapped(realign_kernel<uint16_t>, grid, threads, 0, 1, st, copies[0], copies[1], a.in_features);
+                ? launch_overlapped(realign_kernel<uint8_t>, grid, threads, 0, 1, st, copies[0], copies[1], a.in_features)
+                : launch_overlapped(realign_kernel<uint16_t>, grid, threads, 0, 1, st, copies[0], copies[1], a.in_features);
         if (e != cudaSuccess) return KDA_ERR_LAUNCH;
     }
     const int es = element_bytes(a.in_dtype);
     Plan plan = {};
-    plan.k_blocks = (a.in_features + kRowBytes / es - 1) / (kRowBytes / es);
-    const Choice c = choose(a, plan.k_blocks);
-    const int tile_t = c.pair ? 256 : c.tile, tile_n = c.pair ? c.tile : kLanes;
+    plan.k_blocks = k_blocks;
+    const bool pair = c.kernel == KDA_LINEAR_PAIR;
+    const int tile_t = pair ? 256 : c.tile, tile_n = pair ? c.tile : kLanes;
     plan.tiles_t = (a.num_tokens + tile_t - 1) / tile_t;
     plan.tiles_n = (a.out_features + tile_n - 1) / tile_n;
     plan.out_tma = tma_rows(a.out, a.out_row_stride, a.num_tokens, a.out_features, 2);
@@ -1041,24 +1042,52 @@ extern "C" int kda_linear_launch(const KdaLinearArgs *args, void *workspace, siz
     plan.vectors = ((reinterpret_cast<uintptr_t>(a.bias) | reinterpret_cast<uintptr_t>(a.weight_scale)) & 15u) == 0;
     Maps maps = {};
     bool ok = encode(&maps.x, a.x, a.in_dtype, a.num_tokens, a.in_features,
-                     map_stride(a.x_row_stride, a.num_tokens, a.in_features, es), c.pair ? kLanes : c.tile) &&
+                     map_stride(a.x_row_stride, a.num_tokens, a.in_features, es), pair ? kLanes : c.tile) &&
               encode(&maps.weight, a.weight, a.in_dtype, a.out_features, a.in_features,
-                     map_stride(a.weight_row_stride, a.out_features, a.in_features, es), c.pair ? c.tile / 2 : kLanes);
-    if (c.pair && plan.out_tma)
+                     map_stride(a.weight_row_stride, a.out_features, a.in_features, es), pair ? c.tile / 2 : kLanes);
+    if (pair && plan.out_tma)
         ok = ok && encode(&maps.out, a.out, a.out_dtype, a.num_tokens, a.out_features,
                           map_stride(a.out_row_stride, a.num_tokens, a.out_features, 2), 32);
-    if (c.pair && plan.residual_tma)
+    if (pair && plan.residual_tma)
         ok = ok && encode(&maps.residual, a.residual, a.out_dtype, a.num_tokens, a.out_features,
                           map_stride(a.residual_row_stride, a.num_tokens, a.out_features, 2), 32);
     if (!ok) return KDA_ERR_LAUNCH;
     cudaError_t e;
     if (a.in_dtype == KDA_DTYPE_BF16)
-        e = launch_choice<__nv_bfloat16, false>(a, plan, c, maps, st);
+        e = launch_form<__nv_bfloat16, false>(a, plan, c, maps, st);
     else if (a.in_dtype == KDA_DTYPE_FP16)
-        e = launch_choice<__half, false>(a, plan, c, maps, st);
+        e = launch_form<__half, false>(a, plan, c, maps, st);
     else if (a.out_dtype == KDA_DTYPE_BF16)
-        e = launch_choice<__nv_bfloat16, true>(a, plan, c, maps, st);
+        e = launch_form<__nv_bfloat16, true>(a, plan, c, maps, st);
     else
-        e = launch_choice<__half, true>(a, plan, c, maps, st);
+        e = launch_form<__half, true>(a, plan, c, maps, st);
     return e == cudaSuccess ? KDA_OK : KDA_ERR_LAUNCH;
+}
+
+}  // namespace linear
+}  // namespace kda
+
+extern "C" size_t kda_linear_workspace_bytes(const KdaLinearArgs *args) {
+    using namespace kda::linear;
+    if (check(args) != KDA_OK || args->num_tokens == 0 || args->out_features == 0) return 0;
+    return workspace_bytes_of(*args);
+}
+
+extern "C" int kda_linear_launch(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes, void *stream) {
+    return kda::linear::launch(args, workspace, workspace_bytes, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int kda_linear_form(const KdaLinearArgs *args, int32_t sms, KdaLinearForm *form) {
+    using namespace kda::linear;
+    const int rc = check(args);
+    if (rc != KDA_OK) return rc;
+    if (sms < 0 || form == nullptr || args->num_tokens == 0 || args->out_features == 0) return KDA_ERR_INVALID_ARGUMENT;
+    *form = choose(*args, k_blocks_of(*args), sms > 0 ? sms : kda::sm_count());
+    return KDA_OK;
+}
+
+extern "C" int kda_linear_launch_form(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes,
+                                      const KdaLinearForm *form, void *stream) {
+    if (form == nullptr) return KDA_ERR_INVALID_ARGUMENT;
+    return kda::linear::launch(args, workspace, workspace_bytes, form, static_cast<cudaStream_t>(stream));
 }

@@ -27,6 +27,7 @@ KDA_CHUNK_AUTO, KDA_CHUNK_FUSED, KDA_CHUNK_SPLIT = 0, 1, 2
 KDA_CONV_ACT_NONE, KDA_CONV_ACT_SILU = 0, 1
 KDA_DTYPE_BF16, KDA_DTYPE_FP16, KDA_DTYPE_E4M3 = 0, 1, 2
 KDA_ACT_NONE, KDA_ACT_SILU, KDA_ACT_SIGMOID, KDA_ACT_RELU, KDA_ACT_GELU_TANH = range(5)
+KDA_LINEAR_NARROW, KDA_LINEAR_PAIR = 0, 1
 
 # Entry points declared in include/kda_b200.h.
 EXPORTED = (
@@ -47,6 +48,8 @@ EXPORTED = (
     "kda_gated_rmsnorm_launch",
     "kda_linear_workspace_bytes",
     "kda_linear_launch",
+    "kda_linear_form",
+    "kda_linear_launch_form",
 )
 
 
@@ -199,6 +202,14 @@ class KdaLinearArgs(ctypes.Structure):
     ]
 
 
+class KdaLinearForm(ctypes.Structure):
+    _fields_ = [
+        ("kernel", ctypes.c_int32),
+        ("tile", ctypes.c_int32),
+        ("splits", ctypes.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -242,6 +253,11 @@ def lib() -> ctypes.CDLL:
         L.kda_linear_launch.restype = ctypes.c_int
         L.kda_linear_launch.argtypes = [ctypes.POINTER(KdaLinearArgs), ctypes.c_void_p, ctypes.c_size_t,
                                         ctypes.c_void_p]
+        L.kda_linear_form.restype = ctypes.c_int
+        L.kda_linear_form.argtypes = [ctypes.POINTER(KdaLinearArgs), ctypes.c_int32, ctypes.POINTER(KdaLinearForm)]
+        L.kda_linear_launch_form.restype = ctypes.c_int
+        L.kda_linear_launch_form.argtypes = [ctypes.POINTER(KdaLinearArgs), ctypes.c_void_p, ctypes.c_size_t,
+                                             ctypes.POINTER(KdaLinearForm), ctypes.c_void_p]
         L.kda_chunk_launch_phases.restype = ctypes.c_int
         L.kda_chunk_launch_phases.argtypes = [ctypes.POINTER(KdaArgs), ctypes.c_void_p, ctypes.c_size_t,
                                               ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p), ctypes.c_int]

@@ -449,6 +449,27 @@ typedef struct KdaLinearArgs {
 size_t kda_linear_workspace_bytes(const KdaLinearArgs *args);
 int kda_linear_launch(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes, void *stream);
 
+/* Which kernel a projection takes. */
+typedef enum KdaLinearKernel {
+    KDA_LINEAR_NARROW = 0,   /* few tokens: 128 outputs x `tile` (16, 32, 64) tokens, K over `splits` (1..8) CTAs */
+    KDA_LINEAR_PAIR = 1      /* many tokens: 256 tokens x `tile` (64, 128, 192, 256) outputs per CTA pair, splits 1 */
+} KdaLinearKernel;
+
+typedef struct KdaLinearForm {
+    int32_t kernel;          /* KdaLinearKernel */
+    int32_t tile;
+    int32_t splits;
+} KdaLinearForm;
+
+/* Verification hooks. kda_linear_form: the form that kda_linear_launch takes
+ * for these arguments (T, N >= 1) on a GPU of `sms` SMs (0: the current one);
+ * launches nothing. kda_linear_launch_form: kda_linear_launch with the form given, which
+ * any arguments may take; KDA_ERR_INVALID_ARGUMENT for none of the above, or for
+ * more splits than K has blocks of 128 bytes. */
+int kda_linear_form(const KdaLinearArgs *args, int32_t sms, KdaLinearForm *form);
+int kda_linear_launch_form(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes,
+                           const KdaLinearForm *form, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
