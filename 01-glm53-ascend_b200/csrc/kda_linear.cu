@@ -583,15 +583,15 @@ constexpr int kAhead = 4;
 // the CTA that joins the token, which costs operand stages for an inbox but only one
 // barrier. Otherwise a CTA's sums stay where its stages were and the joining
 // CTA loads them, with a barrier on both sides. Sending pays where each CTA
-// joins few tokens (bf16, K = 4096, tile/splits: 1 token, N = 4096, 16/4 8.2 us
-// against 9.3; 64 tokens, 16/2 13.0 against 13.5, 32/4 12.1 against 12.9; 128
-// tokens, 32/2 15.6 against 14.4; N = 12576, 64 tokens, 64/2 25.9 against 23.6).
+// joins 8 tokens at most, which the rule below gives with 16 tokens a tile only
+// (bf16, K = 4096, N = 4096, tile/splits: 1 token, 16/4 8.2 us against 9.3; 64
+// tokens, 16/2 13.0 against 13.5; 128 tokens, 32/2 15.6 against 14.4).
 template <int BT, bool SEND>
 struct Narrow {
     static constexpr int kBytesW = kLanes * kRowBytes;
     static constexpr int kBytesX = BT * kRowBytes;
     static constexpr int kStageBytes = kBytesW + kBytesX;
-    static constexpr int kStages = (BT <= 16 ? 6 : BT <= 32 ? 5 : 4) - (SEND ? 1 : 0);
+    static constexpr int kStages = BT <= 16 ? (SEND ? 5 : 6) : BT <= 32 ? 5 : 4;
     static constexpr int kThreads = 32 * 6;                   // 4 epilogue warps, loads, products
     static constexpr int kColumns = BT < 32 ? 32 : BT;
     static constexpr int kMaxSplits = 8;
@@ -959,13 +959,10 @@ cudaError_t launch_form(const KdaLinearArgs &a, Plan plan, const KdaLinearForm &
         const bool tma_rows = plan.out_tma && (a.residual == nullptr || plan.residual_tma);
         return tma_rows ? launch_pair<O, E4M3, true>(a, plan, maps, st) : launch_pair<O, E4M3, false>(a, plan, maps, st);
     }
-    const bool send = c.tile <= 8 * c.splits;   // a CTA joins 8 tokens at most
     if (c.tile == 16)
-        return send ? launch_narrow<O, E4M3, 16, true>(a, plan, c.splits, maps, st)
-                    : launch_narrow<O, E4M3, 16, false>(a, plan, c.splits, maps, st);
-    if (c.tile == 32)
-        return send ? launch_narrow<O, E4M3, 32, true>(a, plan, c.splits, maps, st)
-                    : launch_narrow<O, E4M3, 32, false>(a, plan, c.splits, maps, st);
+        return c.splits > 1 ? launch_narrow<O, E4M3, 16, true>(a, plan, c.splits, maps, st)
+                            : launch_narrow<O, E4M3, 16, false>(a, plan, c.splits, maps, st);
+    if (c.tile == 32) return launch_narrow<O, E4M3, 32, false>(a, plan, c.splits, maps, st);
     return launch_narrow<O, E4M3, 64, false>(a, plan, c.splits, maps, st);
 }
 

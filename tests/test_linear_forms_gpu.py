@@ -117,7 +117,7 @@ def test_pair_many_tiles(types, width):
             check((PAIR, width, 1), x, w, s, out, "sigmoid", bias, r)
 
 
-@pytest.mark.parametrize("tile,splits", [(16, 1), (16, 2), (16, 3), (16, 5), (16, 8), (32, 1), (32, 2), (32, 3), (64, 1), (64, 2),
+@pytest.mark.parametrize("tile,splits", [(16, 1), (16, 2), (16, 3), (16, 5), (16, 8), (32, 1), (32, 2), (32, 3), (32, 6), (64, 1), (64, 2),
                                          (64, 3), (64, 8)])
 @pytest.mark.parametrize("types", TYPES)
 def test_narrow(types, tile, splits):
