@@ -123,7 +123,7 @@ __device__ __forceinline__ float e4m3_inverse(float top, float *scale, int64_t r
 // the rows of every tensor start the same `shift` elements past 16 bytes (as
 // contiguous rows of an odd length do), so vectors on 16 bytes cover them with a
 // part of one at either end. LOOSE: single elements, side by side.
-enum Rows { ALIGNED, SHIFTED, LOOSE };
+enum Rows { ALIGNED = KDA_NORM_ALIGNED, SHIFTED = KDA_NORM_SHIFTED, LOOSE = KDA_NORM_LOOSE };
 
 // Elements [e, e + 8) of a row of `columns`, those inside it; zeros for the rest.
 template <typename T>
@@ -718,7 +718,7 @@ struct Layout {
     int rows;       // per CTA
     unsigned grid;
 };
-Layout layout(int64_t units, int64_t rows, int most = 4) {
+Layout layout(int64_t units, int64_t rows, int64_t sms, int most = 4) {
     Layout l = {};
     // As many threads as the rows have units while they fit the GPU at half
     // occupancy, for latency; beyond that more units per thread, which leaves
@@ -726,13 +726,13 @@ Layout layout(int64_t units, int64_t rows, int most = 4) {
     // unit against 6.3 with four; 1,000 rows 8.3 against 6.4).
     int v = 1;
     while (v < 4 && (units > static_cast<int64_t>(v) * kMaxThreads ||
-                     (v < most && units * rows > static_cast<int64_t>(v) * 1024 * sm_count())))
+                     (v < most && units * rows > static_cast<int64_t>(v) * 1024 * sms)))
         v *= 2;
     if (units > static_cast<int64_t>(v) * kMaxThreads) return l;
     while (v > 1 && units <= static_cast<int64_t>(v / 2) * 32) v /= 2;   // one warp, no idle vectors
     l.v = v;
     l.warps = static_cast<int>((units + 32 * v - 1) / (32 * v));
-    l.rows = l.warps >= 4 || rows <= 4 * sm_count() ? 1 : 4 / l.warps;
+    l.rows = l.warps >= 4 || rows <= 4 * sms ? 1 : 4 / l.warps;
     l.grid = static_cast<unsigned>((rows + l.rows - 1) / l.rows);
     return l;
 }
@@ -746,7 +746,7 @@ struct RingLayout {
     unsigned grid;
     RingPlan plan;
 };
-RingLayout ring_layout(int64_t units, int64_t rows, int inputs) {
+RingLayout ring_layout(int64_t units, int64_t rows, int inputs, int64_t sms) {
     RingLayout l = {};
     int v = 4;
     while (v > 1 && units <= static_cast<int64_t>(v / 2) * 32) v /= 2;
@@ -755,7 +755,7 @@ RingLayout ring_layout(int64_t units, int64_t rows, int inputs) {
     l.plan.warps = static_cast<int>(warps);
     l.plan.rows = warps >= 4 ? 1 : static_cast<int>(4 / warps);
     const int per_sm = kRingWarps / (l.plan.warps * l.plan.rows) > 0 ? kRingWarps / (l.plan.warps * l.plan.rows) : 1;
-    const int64_t grid = static_cast<int64_t>(per_sm) * sm_count();
+    const int64_t grid = per_sm * sms;
     if (rows < 3 * grid * l.plan.rows) return l;
     l.plan.row_bytes = static_cast<int32_t>(units * 16);
     const int stage = l.plan.rows * inputs * l.plan.row_bytes;
@@ -801,27 +801,55 @@ cudaError_t launch_ring(const KdaNormArgs &a, const RingLayout &r, cudaStream_t 
            : r.v == 2 ? launch_ring_v<T, FP8, RESIDUAL, 2>(a, r, st)
                       : launch_ring_v<T, FP8, RESIDUAL, 4>(a, r, st);
 }
-template <typename T, bool FP8>
-cudaError_t launch(const KdaNormArgs &a, cudaStream_t st) {
+// What a launch takes: the ring (ring.v != 0), the direct kernel (direct.v != 0), or neither: rows read twice.
+struct Plan {
+    Rows rows;
+    RingLayout ring;
+    Layout direct;
+};
+Plan plan_of(const KdaNormArgs &a, int64_t sms) {
     const int64_t T_ = a.num_tokens;
     const bool res = a.residual != nullptr, res_out = res && a.residual_out != nullptr;
     // Bases on 16 bytes (8 for e4m3), and the rows' distances alike modulo 8 elements.
     const bool based = aligned(a.x, 0, 1, 2) && (!res || aligned(a.residual, 0, 1, 2)) &&
-                       (!res_out || aligned(a.residual_out, 0, 1, 2)) && aligned_out(a.out, 0, 1, FP8);
+                       (!res_out || aligned(a.residual_out, 0, 1, 2)) && aligned_out(a.out, 0, 1, a.scale != nullptr);
     const int64_t stride = T_ > 1 ? a.x_row_stride : 0;
     const auto alike = [&](int64_t other) { return T_ <= 1 || (stride - other) % 8 == 0; };
     const bool same = based && alike(a.out_row_stride) && (!res || alike(a.residual_row_stride)) &&
                       (!res_out || alike(a.residual_out_row_stride));
-    const Rows rows = !same ? LOOSE : a.hidden % 8 == 0 && stride % 8 == 0 && aligned(a.weight, 0, 1, 4) ? ALIGNED : SHIFTED;
-    const int64_t units = (static_cast<int64_t>(a.hidden) + 7) / 8 + (rows == SHIFTED ? 1 : 0);   // a part at either end
-    if (rows == ALIGNED) {
-        const RingLayout r = ring_layout(units, T_, res ? 2 : 1);
-        if (r.v != 0) return res ? launch_ring<T, FP8, true>(a, r, st) : launch_ring<T, FP8, false>(a, r, st);
-    }
-    const Layout l = layout(units, T_, rows == ALIGNED ? 4 : 2);   // the other forms hold more registers per unit
-    if (l.v == 0)
-        return launch_overlapped(rmsnorm_long_kernel<T, FP8>, dim3(static_cast<unsigned>(T_)), kLongThreads, 0, 1, st, a);
-    return res ? launch_rows<T, FP8, true>(rows, a, l, st) : launch_rows<T, FP8, false>(rows, a, l, st);
+    Plan p = {};
+    p.rows = !same ? LOOSE : a.hidden % 8 == 0 && stride % 8 == 0 && aligned(a.weight, 0, 1, 4) ? ALIGNED : SHIFTED;
+    const int64_t units = (static_cast<int64_t>(a.hidden) + 7) / 8 + (p.rows == SHIFTED ? 1 : 0);   // a part at either end
+    if (p.rows == ALIGNED) p.ring = ring_layout(units, T_, res ? 2 : 1, sms);
+    if (p.ring.v == 0) p.direct = layout(units, T_, sms, p.rows == ALIGNED ? 4 : 2);   // the other forms hold more registers per unit
+    if (p.ring.v == 0 && p.direct.v == 0) p.rows = LOOSE;
+    return p;
+}
+template <typename T, bool FP8>
+cudaError_t launch(const KdaNormArgs &a, cudaStream_t st) {
+    const bool res = a.residual != nullptr;
+    const Plan p = plan_of(a, sm_count());
+    if (p.ring.v != 0) return res ? launch_ring<T, FP8, true>(a, p.ring, st) : launch_ring<T, FP8, false>(a, p.ring, st);
+    if (p.direct.v == 0)
+        return launch_overlapped(rmsnorm_long_kernel<T, FP8>, dim3(static_cast<unsigned>(a.num_tokens)), kLongThreads, 0, 1, st, a);
+    return res ? launch_rows<T, FP8, true>(p.rows, a, p.direct, st) : launch_rows<T, FP8, false>(p.rows, a, p.direct, st);
+}
+
+Plan plan_of(const KdaGatedNormArgs &a, int64_t sms) {
+    const int64_t T_ = a.num_tokens, units = static_cast<int64_t>(a.num_heads) * (a.head_dim / 8);
+    const bool vec = aligned(a.o, a.o_stride[0], T_, 2) && aligned(a.o, a.o_stride[1], a.num_heads, 2) &&
+                     aligned(a.gate, a.gate_row_stride, T_, 2) && aligned_out(a.out, a.out_row_stride, T_, a.scale != nullptr);
+    Plan p = {};
+    p.rows = vec ? ALIGNED : LOOSE;
+    // The ring copies a token's heads as one row.
+    if (vec && (a.num_heads == 1 || a.o_stride[1] == a.head_dim)) p.ring = ring_layout(units, T_, 2, sms);
+    if (p.ring.v == 0) p.direct = layout(units, T_, sms);
+    return p;
+}
+KdaNormForm form_of(const Plan &p) {
+    if (p.ring.v != 0) return {KDA_NORM_RING, p.rows, p.ring.v, p.ring.plan.warps};
+    if (p.direct.v != 0) return {KDA_NORM_DIRECT, p.rows, p.direct.v, p.direct.warps};
+    return {KDA_NORM_LONG, p.rows, 0, kLongThreads / 32};
 }
 
 template <typename T, bool FP8, int D, int ACT, int V>
@@ -832,20 +860,15 @@ cudaError_t launch_gated_ring(const KdaGatedNormArgs &a, const RingLayout &r, cu
 }
 template <typename T, bool FP8, int D, int ACT>
 cudaError_t launch_gated(const KdaGatedNormArgs &a, cudaStream_t st) {
-    const int64_t T_ = a.num_tokens, units = static_cast<int64_t>(a.num_heads) * (D / 8);
-    const bool vec = aligned(a.o, a.o_stride[0], T_, 2) && aligned(a.o, a.o_stride[1], a.num_heads, 2) &&
-                     aligned(a.gate, a.gate_row_stride, T_, 2) && aligned_out(a.out, a.out_row_stride, T_, FP8);
-    // The ring copies a token's heads as one row.
-    if (vec && (a.num_heads == 1 || a.o_stride[1] == D)) {
-        const RingLayout r = ring_layout(units, T_, 2);
-        if (r.v == 1) return launch_gated_ring<T, FP8, D, ACT, 1>(a, r, st);
-        if (r.v == 2) return launch_gated_ring<T, FP8, D, ACT, 2>(a, r, st);
-        if (r.v == 4) return launch_gated_ring<T, FP8, D, ACT, 4>(a, r, st);
-    }
-    const Layout l = layout(units, T_);
+    const Plan p = plan_of(a, sm_count());
+    const bool vec = p.rows == ALIGNED;
+    if (p.ring.v == 1) return launch_gated_ring<T, FP8, D, ACT, 1>(a, p.ring, st);
+    if (p.ring.v == 2) return launch_gated_ring<T, FP8, D, ACT, 2>(a, p.ring, st);
+    if (p.ring.v == 4) return launch_gated_ring<T, FP8, D, ACT, 4>(a, p.ring, st);
+    const Layout &l = p.direct;
     if (l.v == 0)
-        return launch_overlapped(gated_rmsnorm_long_kernel<T, FP8, D, ACT>, dim3(static_cast<unsigned>(T_)), kLongThreads, 0, 1,
-                                 st, a, vec);
+        return launch_overlapped(gated_rmsnorm_long_kernel<T, FP8, D, ACT>, dim3(static_cast<unsigned>(a.num_tokens)),
+                                 kLongThreads, 0, 1, st, a, vec);
     const auto kernel = l.v == 1   ? gated_rmsnorm_kernel<T, FP8, D, ACT, 1>
                         : l.v == 2 ? gated_rmsnorm_kernel<T, FP8, D, ACT, 2>
                                    : gated_rmsnorm_kernel<T, FP8, D, ACT, 4>;
@@ -861,11 +884,8 @@ cudaError_t launch_gated(const KdaGatedNormArgs &a, cudaStream_t st) {
 
 bool stride_ok(int64_t stride, int64_t columns, int64_t rows) { return rows <= 1 || stride >= columns; }
 
-}  // namespace norm
-}  // namespace kda
-
-extern "C" int kda_rmsnorm_launch(const KdaNormArgs *args, void *stream) {
-    using namespace kda::norm;
+// Argument checks of the two launchers: KDA_OK, or the code to return.
+int check(const KdaNormArgs *args) {
     if (args == nullptr) return KDA_ERR_INVALID_ARGUMENT;
     const KdaNormArgs &a = *args;
     if (a.num_tokens < 0 || a.hidden <= 0) return KDA_ERR_INVALID_ARGUMENT;
@@ -875,16 +895,9 @@ extern "C" int kda_rmsnorm_launch(const KdaNormArgs *args, void *stream) {
     if (!stride_ok(a.out_row_stride, a.hidden, a.num_tokens) ||
         (a.residual_out != nullptr && !stride_ok(a.residual_out_row_stride, a.hidden, a.num_tokens)))
         return KDA_ERR_INVALID_ARGUMENT;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool fp8 = a.scale != nullptr;
-    const cudaError_t e = a.dtype == KDA_DTYPE_BF16
-                              ? (fp8 ? launch<__nv_bfloat16, true>(a, st) : launch<__nv_bfloat16, false>(a, st))
-                              : (fp8 ? launch<__half, true>(a, st) : launch<__half, false>(a, st));
-    return e == cudaSuccess ? KDA_OK : KDA_ERR_LAUNCH;
+    return KDA_OK;
 }
-
-extern "C" int kda_gated_rmsnorm_launch(const KdaGatedNormArgs *args, void *stream) {
-    using namespace kda::norm;
+int check(const KdaGatedNormArgs *args) {
     if (args == nullptr) return KDA_ERR_INVALID_ARGUMENT;
     const KdaGatedNormArgs &a = *args;
     if (a.num_tokens < 0 || a.num_heads <= 0) return KDA_ERR_INVALID_ARGUMENT;
@@ -896,10 +909,50 @@ extern "C" int kda_gated_rmsnorm_launch(const KdaGatedNormArgs *args, void *stre
     if (a.o == nullptr || a.gate == nullptr || a.weight == nullptr || a.out == nullptr) return KDA_ERR_INVALID_ARGUMENT;
     if (!stride_ok(a.out_row_stride, static_cast<int64_t>(a.num_heads) * a.head_dim, a.num_tokens))
         return KDA_ERR_INVALID_ARGUMENT;
+    return KDA_OK;
+}
+template <typename Args>
+int form_of(const Args *args, int32_t sms, KdaNormForm *form) {
+    const int rc = check(args);
+    if (rc != KDA_OK) return rc;
+    if (sms < 0 || form == nullptr || args->num_tokens == 0) return KDA_ERR_INVALID_ARGUMENT;
+    *form = form_of(plan_of(*args, sms > 0 ? sms : sm_count()));
+    return KDA_OK;
+}
+
+}  // namespace norm
+}  // namespace kda
+
+extern "C" int kda_rmsnorm_launch(const KdaNormArgs *args, void *stream) {
+    using namespace kda::norm;
+    const int rc = check(args);
+    if (rc != KDA_OK || args->num_tokens == 0) return rc;
+    const KdaNormArgs &a = *args;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool fp8 = a.scale != nullptr;
+    const cudaError_t e = a.dtype == KDA_DTYPE_BF16
+                              ? (fp8 ? launch<__nv_bfloat16, true>(a, st) : launch<__nv_bfloat16, false>(a, st))
+                              : (fp8 ? launch<__half, true>(a, st) : launch<__half, false>(a, st));
+    return e == cudaSuccess ? KDA_OK : KDA_ERR_LAUNCH;
+}
+
+extern "C" int kda_gated_rmsnorm_launch(const KdaGatedNormArgs *args, void *stream) {
+    using namespace kda::norm;
+    const int rc = check(args);
+    if (rc != KDA_OK || args->num_tokens == 0) return rc;
+    const KdaGatedNormArgs &a = *args;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool bf16 = a.dtype == KDA_DTYPE_BF16;
     const cudaError_t e =
         a.head_dim == 128 ? (bf16 ? launch_gated<__nv_bfloat16, 128>(a, st) : launch_gated<__half, 128>(a, st))
                           : (bf16 ? launch_gated<__nv_bfloat16, 64>(a, st) : launch_gated<__half, 64>(a, st));
     return e == cudaSuccess ? KDA_OK : KDA_ERR_LAUNCH;
+}
+
+extern "C" int kda_rmsnorm_form(const KdaNormArgs *args, int32_t sms, KdaNormForm *form) {
+    return kda::norm::form_of(args, sms, form);
+}
+
+extern "C" int kda_gated_rmsnorm_form(const KdaGatedNormArgs *args, int32_t sms, KdaNormForm *form) {
+    return kda::norm::form_of(args, sms, form);
 }

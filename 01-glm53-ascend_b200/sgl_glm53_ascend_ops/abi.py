@@ -27,6 +27,8 @@ KDA_CHUNK_AUTO, KDA_CHUNK_FUSED, KDA_CHUNK_SPLIT = 0, 1, 2
 KDA_CONV_ACT_NONE, KDA_CONV_ACT_SILU = 0, 1
 KDA_DTYPE_BF16, KDA_DTYPE_FP16, KDA_DTYPE_E4M3 = 0, 1, 2
 KDA_ACT_NONE, KDA_ACT_SILU, KDA_ACT_SIGMOID, KDA_ACT_RELU, KDA_ACT_GELU_TANH = range(5)
+KDA_NORM_DIRECT, KDA_NORM_RING, KDA_NORM_LONG = 0, 1, 2
+KDA_NORM_ALIGNED, KDA_NORM_SHIFTED, KDA_NORM_LOOSE = 0, 1, 2
 KDA_LINEAR_NARROW, KDA_LINEAR_PAIR = 0, 1
 
 # Entry points declared in include/kda_b200.h.
@@ -46,6 +48,8 @@ EXPORTED = (
     "kda_conv_launch",
     "kda_rmsnorm_launch",
     "kda_gated_rmsnorm_launch",
+    "kda_rmsnorm_form",
+    "kda_gated_rmsnorm_form",
     "kda_linear_workspace_bytes",
     "kda_linear_launch",
     "kda_linear_form",
@@ -179,6 +183,15 @@ class KdaGatedNormArgs(ctypes.Structure):
     ]
 
 
+class KdaNormForm(ctypes.Structure):
+    _fields_ = [
+        ("kernel", ctypes.c_int32),
+        ("rows", ctypes.c_int32),
+        ("units", ctypes.c_int32),
+        ("warps", ctypes.c_int32),
+    ]
+
+
 class KdaLinearArgs(ctypes.Structure):
     _fields_ = [
         ("x", ctypes.c_void_p),
@@ -248,6 +261,9 @@ def lib() -> ctypes.CDLL:
         L.kda_rmsnorm_launch.argtypes = [ctypes.POINTER(KdaNormArgs), ctypes.c_void_p]
         L.kda_gated_rmsnorm_launch.restype = ctypes.c_int
         L.kda_gated_rmsnorm_launch.argtypes = [ctypes.POINTER(KdaGatedNormArgs), ctypes.c_void_p]
+        for name, args_type in (("kda_rmsnorm_form", KdaNormArgs), ("kda_gated_rmsnorm_form", KdaGatedNormArgs)):
+            getattr(L, name).restype = ctypes.c_int
+            getattr(L, name).argtypes = [ctypes.POINTER(args_type), ctypes.c_int32, ctypes.POINTER(KdaNormForm)]
         L.kda_linear_workspace_bytes.restype = ctypes.c_size_t
         L.kda_linear_workspace_bytes.argtypes = [ctypes.POINTER(KdaLinearArgs)]
         L.kda_linear_launch.restype = ctypes.c_int

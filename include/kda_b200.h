@@ -417,6 +417,31 @@ typedef struct KdaGatedNormArgs {
 
 int kda_gated_rmsnorm_launch(const KdaGatedNormArgs *args, void *stream);
 
+/* Which kernel a norm takes, and how its rows lie. */
+typedef enum KdaNormKernel {
+    KDA_NORM_DIRECT = 0,     /* a row on 1..32 warps, held in registers */
+    KDA_NORM_RING = 1,       /* many rows: persistent CTAs fed by a ring of copies */
+    KDA_NORM_LONG = 2        /* rows too long for registers, read twice */
+} KdaNormKernel;
+
+typedef enum KdaNormRows {
+    KDA_NORM_ALIGNED = 0,    /* vectors of 8 elements on 16 bytes */
+    KDA_NORM_SHIFTED = 1,    /* rmsnorm: every tensor's row starts alike past 16 bytes; vectors with a part at either end */
+    KDA_NORM_LOOSE = 2       /* single elements */
+} KdaNormRows;
+
+typedef struct KdaNormForm {
+    int32_t kernel;          /* KdaNormKernel */
+    int32_t rows;            /* KdaNormRows; of KDA_NORM_LONG rmsnorm always KDA_NORM_LOOSE */
+    int32_t units;           /* 8-element units a thread: 1, 2 or 4; 0 of KDA_NORM_LONG */
+    int32_t warps;           /* per row */
+} KdaNormForm;
+
+/* Verification hooks: the form a launch takes for these arguments on a GPU of
+ * `sms` SMs (0: the current one). They launch nothing. */
+int kda_rmsnorm_form(const KdaNormArgs *args, int32_t sms, KdaNormForm *form);
+int kda_gated_rmsnorm_form(const KdaGatedNormArgs *args, int32_t sms, KdaNormForm *form);
+
 /* A projection with its epilogue:
  *   out[t, n] = round(act(x_scale[t] * (weight_scale[n] * sum_k x[t, k] * weight[n, k]) + bias[n]) + residual[t, n])
  * fp32 sums, the scales multiplied in that order. x and weight are of one type:
