@@ -68,8 +68,9 @@ __device__ __forceinline__ uint32_t pack4_e4m3(float a, float b, float c, float 
 }
 
 // 1 / (1 + e^-z) of a pair by the hardware's approximate 2^x and reciprocal: 2^-22
-// of itself plus 2^-24 |z| from the rounding of z log2(e). Goes to 0 and 1
-// where e^-z leaves fp32's range; NaN stays NaN.
+// of itself plus 2^-24 |z| from the rounding of z log2(e), for z > -87.3. Below, where
+// it is smaller than fp32's smallest normal value (2^-126), it goes to 0, and with it
+// y / (1 + e^-z), by 88 * 2^-126 at most; above it goes to 1. NaN stays NaN.
 __device__ __forceinline__ float exp2_approx(float z) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(z));
