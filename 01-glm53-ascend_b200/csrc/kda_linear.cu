@@ -12,14 +12,15 @@
 //     output's bytes for short K. A tile of 256 x 256 brings 32 KB to each SM per
 //     128-byte block of K and its 512 cycles of products; two accumulators let the
 //     next tile's products run under the epilogue. 8256 x 12576 x 4096 bf16:
-//     1,300 TFLOP/s at the power limit (the tensor pipe 92% active on 4096 x
+//     1,300 TFLOP/s at the power limit (the tensor pipe 90% active on 4096 x
 //     9216); 33494 x 4096 x 4096 e4m3 with residual: 2,300 TFLOP/s.
 //   * narrow_kernel, for few tokens, where the weights' bytes are the work:
 //     128 outputs on the lanes x 16..64 tokens as the columns, so that a tile of
 //     weights is read once; K split over the CTAs of a cluster, which keeps every
 //     SM reading, and joined through distributed shared memory in a fixed order, so
-//     results repeat bit for bit. 64 x 12576 x 4096 bf16: 23.4 us, for 14.7 us of
-//     them the weights arriving at 7 TB/s.
+//     results repeat bit for bit. 64 x 12576 x 4096 bf16 with weights that no
+//     earlier launch left in L2: 22.9 us, 4.5 TB/s; 1 x 4096 x 4096 e4m3: 6.2 us, of
+//     which the weights' bytes are 2.6 at HBM's rate, the rest first load, join and launch.
 // Operands whose rows do not start on 16-byte boundaries, which TMA needs, are
 // first copied to rows that do (realign_kernel).
 
@@ -281,7 +282,9 @@ struct Pair {
 };
 
 // Tile `i` in an order that keeps the operands of the tiles in flight few:
-// strips of 8 token tiles, the token tile running fastest.
+// strips of 8 token tiles, the token tile running fastest. 33494 x 12576 x 4096
+// e4m3: 1,415 us in strips of 1, 2 or 4, 1,367 of 8, 1,362 of 16, 1,372 of 32; 33494 x
+// 4096 x 4096 436 up to 8, 441 beyond.
 __device__ __forceinline__ void tile_at(int i, int tiles_t, int tiles_n, int &t, int &n) {
     constexpr int kStrip = 8;
     const int strip = i / (kStrip * tiles_n), first = strip * kStrip;
@@ -891,7 +894,10 @@ bool encode(CUtensorMap *map, const void *base, int32_t dtype, int64_t rows, int
 // tokens: 64/2 23.6, 32/1 26.5, pair 25.4; 128 tokens: 64/1 29.6, pair 27.8.
 // Otherwise the pair kernel, with the width whose waves of tiles take the
 // fewest cycles: per tile either its K blocks (measured: 345, 345, 425 and 525
-// cycles at widths 64..256) or its epilogue, whichever is longer. 256 tokens,
+// cycles at widths 64..256) or its epilogue, whichever is longer. What an epilogue
+// takes depends on what is in it (measured at K = 64, bf16, widths 64..256: 2,160 to
+// 3,070 cycles with none, 3,510 to 5,700 with bias and sigmoid, 4,180 to 10,100 with a
+// residual beside); the rule has one figure, between the first two. 256 tokens,
 // N = 12576, K = 4096 e4m3: width 192 (66 tiles) 17.7 us, 256 (50) 19.3, 128 (99)
 // 23.9; 512 tokens, N = 4096 bf16: 128 (64 tiles) 21.7, 256 (32) 27.0.
 KdaLinearForm choose(const KdaLinearArgs &a, int64_t k_blocks, int64_t sms) {

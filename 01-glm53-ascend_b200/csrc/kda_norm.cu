@@ -5,9 +5,11 @@
 //
 // Both read every input once and write every output once (5 to 7 bytes an
 // element against ~10 operations), so HBM bounds them, or latency when there
-// are few rows: 33,494 rows of 4,096 with an e4m3 output take 155 us (rmsnorm
-// with residual, 6.2 TB/s) and 116 us (gated, 5.9 TB/s; its two
-// special-function operations an element take half of that time), 256 rows 4.3 us.
+// are few rows: 33,494 rows of 4,096 with an e4m3 output take 156 us (rmsnorm
+// with residual, 6.2 TB/s) and 114 us (gated, 6.0 TB/s; its two special-function
+// operations an element keep that unit 63% busy), 256 rows 3 to 4 us.
+// Rows off 16 bytes miss the ring, whose copies start on 16 bytes, and read their
+// weights singly: 33,494 x 1,001 fp16 take 55 us (2.4 TB/s).
 // A row belongs to a group of 1..32 warps that keeps all of it in registers;
 // the statistics cross lanes by shuffles and warps by one exchange through
 // shared memory. The e4m3 scale needs max|y| = max|s w| / rms, so rmsnorm

@@ -114,7 +114,9 @@ def kda_layer_extend(
     """One layer's extend (prefill) step over a varlen batch: the residual
     stream hidden [T, N] (or [1, T, N]) bf16, plus ``residual`` where the block
     before hands over two parts, to the stream after the layer. The pools and
-    the other arguments are those of :func:`kda_forward_extend`."""
+    the other arguments are those of :func:`kda_forward_extend`. The output
+    projection adds the stream, so the weights hold all of the layer's heads:
+    results over parts of the heads cannot be summed (each has the stream)."""
     return _layer(kda_forward_extend, hidden, weights, residual, head_dim, conv_state=conv_state,
                   temporal_state=temporal_state, cache_indices=cache_indices, query_start_loc=query_start_loc,
                   scale=scale, has_initial_state=has_initial_state, track_indices=track_indices, track_lens=track_lens)
