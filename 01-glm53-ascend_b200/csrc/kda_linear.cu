@@ -217,7 +217,7 @@ __device__ __forceinline__ void activate_all(int act, float2 (&y)[N]) {
 }
 // v[n .. n + 3] of an fp32 vector of `size` values (zeros past the end), alike in every lane.
 __device__ __forceinline__ float4 vector4(const float *v, int64_t n, int64_t size, bool aligned) {
-    if (aligned && n + 4 <= size) return __ldg(reinterpret_cast<const float4 *>(v + n));
+    if (aligned && n + 4 <= size) return *reinterpret_cast<const float4 *>(v + n);
     return make_float4(n < size ? v[n] : 0.0f, n + 1 < size ? v[n + 1] : 0.0f, n + 2 < size ? v[n + 2] : 0.0f,
                        n + 3 < size ? v[n + 3] : 0.0f);
 }
@@ -473,8 +473,8 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int64_t at = n0 + h * 32 + lane;
-                bias[h] = any && p.bias != nullptr && at < p.out_features ? __ldg(p.bias + at) : 0.0f;
-                scale[h] = E4M3 && any && at < p.out_features ? __ldg(p.weight_scale + at) : 0.0f;
+                bias[h] = any && p.bias != nullptr && at < p.out_features ? p.bias[at] : 0.0f;
+                scale[h] = E4M3 && any && at < p.out_features ? p.weight_scale[at] : 0.0f;
             }
             bool ok = mbar_wait(&tfull[buffer], tphase, p.status, abort_word);
             if (residual_tma && any) {

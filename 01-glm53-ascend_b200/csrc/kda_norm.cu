@@ -9,7 +9,7 @@
 // with residual, 6.2 TB/s) and 114 us (gated, 6.0 TB/s; its two special-function
 // operations an element keep that unit 63% busy), 256 rows 3 to 4 us.
 // Rows off 16 bytes miss the ring, whose copies start on 16 bytes, and read their
-// weights singly: 33,494 x 1,001 fp16 take 55 us (2.4 TB/s).
+// weights singly: 33,494 x 1,001 fp16 take 53 us (2.5 TB/s).
 // A row belongs to a group of 1..32 warps that keeps all of it in registers;
 // the statistics cross lanes by shuffles and warps by one exchange through
 // shared memory. The e4m3 scale needs max|y| = max|s w| / rms, so rmsnorm
@@ -31,7 +31,7 @@ constexpr int kLongThreads = 256;
 
 template <typename T>
 __device__ __forceinline__ float weight_at(const void *w, bool fp32, int64_t i) {
-    return fp32 ? __ldg(static_cast<const float *>(w) + i) : to_f32(static_cast<const T *>(w)[i]);
+    return fp32 ? static_cast<const float *>(w)[i] : to_f32(static_cast<const T *>(w)[i]);
 }
 
 // Sum or maximum over `warps` warps of this thread's row (group `slot` of the
@@ -58,14 +58,10 @@ __device__ __forceinline__ void unpack8(uint4 r, float2 (&v)[4]) {
     v[0] = unpack2<T>(r.x), v[1] = unpack2<T>(r.y), v[2] = unpack2<T>(r.z), v[3] = unpack2<T>(r.w);
 }
 // Eight neighbouring elements of a row as four pairs; one 16-byte access where the row allows it.
-// WRITTEN: the kernel may write over what it reads here (x and residual, which residual_out may
-// be), so the load must not take the read-only path.
-template <typename T, bool WRITTEN = false>
+template <typename T>
 __device__ __forceinline__ void load8(const T *p, bool aligned, float2 (&v)[4]) {
     if (aligned) {
-        const uint4 *at = reinterpret_cast<const uint4 *>(p);
-        const uint4 r = WRITTEN ? *at : __ldg(at);
-        unpack8<T>(r, v);
+        unpack8<T>(*reinterpret_cast<const uint4 *>(p), v);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = make_float2(to_f32(p[2 * i]), to_f32(p[2 * i + 1]));
@@ -106,7 +102,7 @@ template <typename T>
 __device__ __forceinline__ void vector_weights(const KdaNormArgs &p, int e, float2 (&w)[4]) {
     if (p.weight_fp32) {
         const float4 *q = reinterpret_cast<const float4 *>(static_cast<const float *>(p.weight) + e);
-        const float4 a = __ldg(q), b = __ldg(q + 1);
+        const float4 a = q[0], b = q[1];
         w[0] = make_float2(a.x, a.y), w[1] = make_float2(a.z, a.w);
         w[2] = make_float2(b.x, b.y), w[3] = make_float2(b.z, b.w);
     } else {
@@ -159,10 +155,12 @@ constexpr float kDown = 0x1p-32f, kUp = 0x1p32f;
 // `threads` apart, which keeps a warp's 2-byte accesses side by side. The sum
 // with the residual is stored as soon as it is known; until the row's
 // statistics have met, s w is held for an e4m3 output, and s otherwise, with
-// the weights beside it where they are few (loaded afterwards they cost a row alone
-// their latency).
+// the weights beside it, loaded first, where they are few (loaded afterwards they cost
+// a row alone their latency). Rows off 16 bytes get one block of 1024 threads as their
+// bound: left to itself the compiler takes 32 registers for some and spills (1,021 x
+// 1,001 fp16 5.0 us against 3.8).
 template <typename T, bool FP8, bool RESIDUAL, Rows ROWS, int V>
-__global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs p, const int warps) {
+__global__ void __launch_bounds__(kMaxThreads, ROWS == ALIGNED ? 0 : 1) rmsnorm_kernel(const KdaNormArgs p, const int warps) {
     using Out = typename std::conditional<FP8, __nv_fp8_e4m3, T>::type;
     __shared__ float2 part[kMaxThreads / 32];
     let_next_start();
@@ -180,35 +178,6 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs 
     // Unit j of this thread: its first element, or (LOOSE) that of its k-th pair's first half.
     const auto first = [&](int j) { return (j * threads + tid) * 8 - shift; };
     const auto loose = [&](int j, int e) { return (j * 8 + e) * threads + tid; };
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        if (ROWS == LOOSE) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int a = loose(j, 2 * k), b = loose(j, 2 * k + 1);
-                v[j][k] = make_float2(a < columns ? to_f32(x[a]) : 0.0f, b < columns ? to_f32(x[b]) : 0.0f);
-                if (RESIDUAL)
-                    v[j][k] = add2(v[j][k], make_float2(a < columns ? to_f32(res[a]) : 0.0f, b < columns ? to_f32(res[b]) : 0.0f));
-            }
-            continue;
-        }
-        const int e = first(j);
-        const bool whole = ROWS == ALIGNED ? e < columns : e >= 0 && e + 8 <= columns;
-        if (whole) {
-            load8<T, RESIDUAL>(x + e, true, v[j]);
-        } else if (ROWS == SHIFTED && e < columns) {
-            load8_part(x, e, columns, v[j]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[j][k] = make_float2(0.0f, 0.0f);
-        }
-        if (RESIDUAL && (whole || (ROWS == SHIFTED && e < columns))) {
-            float2 r[4];
-            whole ? load8<T, true>(res + e, true, r) : load8_part(res, e, columns, r);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[j][k] = add2(v[j][k], r[k]);
-        }
-    }
     // The weights of unit j; zeros, or (SHIFTED) some weight, past the row's ends. ALIGNED units lie inside it.
     const auto weights = [&](int j, float2 (&w)[4]) {
         if constexpr (ROWS == ALIGNED) {
@@ -228,6 +197,38 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs 
     };
     constexpr bool kHeld = !FP8 && V <= 2;
     float2 held[kHeld ? V : 1][4];
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        if (kHeld && (ROWS != ALIGNED || first(j) < columns)) weights(j, held[j]);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (ROWS == LOOSE) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int a = loose(j, 2 * k), b = loose(j, 2 * k + 1);
+                v[j][k] = make_float2(a < columns ? to_f32(x[a]) : 0.0f, b < columns ? to_f32(x[b]) : 0.0f);
+                if (RESIDUAL)
+                    v[j][k] = add2(v[j][k], make_float2(a < columns ? to_f32(res[a]) : 0.0f, b < columns ? to_f32(res[b]) : 0.0f));
+            }
+            continue;
+        }
+        const int e = first(j);
+        const bool whole = ROWS == ALIGNED ? e < columns : e >= 0 && e + 8 <= columns;
+        if (whole) {
+            load8(x + e, true, v[j]);
+        } else if (ROWS == SHIFTED && e < columns) {
+            load8_part(x, e, columns, v[j]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j][k] = make_float2(0.0f, 0.0f);
+        }
+        if (RESIDUAL && (whole || (ROWS == SHIFTED && e < columns))) {
+            float2 r[4];
+            whole ? load8(res + e, true, r) : load8_part(res, e, columns, r);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j][k] = add2(v[j][k], r[k]);
+        }
+    }
     float top = 0.0f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -250,7 +251,6 @@ __global__ void __launch_bounds__(kMaxThreads) rmsnorm_kernel(const KdaNormArgs 
         }
         float2 w[4];
         if (FP8) weights(j, w);
-        if (kHeld) weights(j, held[j]);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             sum = fma2(v[j][k], v[j][k], sum);
@@ -589,6 +589,8 @@ __global__ void __maxnreg__(kRingRegisters) rmsnorm_ring_kernel(const KdaNormArg
         for (int j = 0; j < V; ++j) {
             const int i = (j * threads + tid) * 8;
             if (live && i < p.hidden) {
+                float2 w[4];
+                if (FP8) vector_weights<T>(p, i, w);   // ahead of the store, which no load passes
                 load8_shared<T>(x + i * 2, v[j]);
                 if (RESIDUAL) {
                     float2 r[4];
@@ -601,8 +603,6 @@ __global__ void __maxnreg__(kRingRegisters) rmsnorm_ring_kernel(const KdaNormArg
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum = fma2(v[j][e], v[j][e], sum);
                 if (FP8) {
-                    float2 w[4];
-                    vector_weights<T>(p, i, w);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[j][e] = mul2(mul2(v[j][e], make_float2(kDown, kDown)), w[e]);
                     top = max8(top, v[j]);

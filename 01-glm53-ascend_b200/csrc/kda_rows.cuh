@@ -106,7 +106,9 @@ __device__ __forceinline__ float2 activate2(float2 y) {
 
 // Programmatic dependent launch: these kernels let the next one in the stream
 // start its set-up while they run, and wait for everything before them ahead
-// of their first access to global memory.
+// of their first access to global memory. What they read may thus be written
+// while they already run, as no memory of the read-only path may: they use
+// ordinary loads (and the async proxy) throughout.
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -146,3 +146,15 @@ def test_schemas_say_which_results_may_be_none():
     ns = torch.ops.sgl_glm53_ascend
     assert str(ns.kda_rmsnorm.default._schema).endswith("bool fp8=False) -> (Tensor, Tensor?, Tensor?)")
     assert str(ns.kda_gated_rmsnorm.default._schema).endswith("bool fp8=False) -> (Tensor, Tensor?)")
+
+
+def test_overlapped_kernels_take_no_read_only_loads():
+    """Kernels that start while the one before them runs (launch_overlapped) may read what that one still writes. The
+    read-only path needs memory that nobody writes for as long as the kernel runs, so their sources do not use it."""
+    sources = sorted((PKG_DIR / "csrc").glob("*.cu"))
+    overlapped = [p for p in sources if "launch_overlapped(" in p.read_text()]
+    assert {p.name for p in overlapped} == {"kda_norm.cu", "kda_linear.cu"}
+    for path in overlapped + [PKG_DIR / "csrc" / "kda_rows.cuh", PKG_DIR / "csrc" / "kda_ring.cuh"]:
+        text = path.read_text()
+        for word in ("__ldg(", "ld.global.nc", "__restrict__", "load_bf16x4(", "load_f32x4("):
+            assert word not in text, f"{path.name}: {word}"
