@@ -47,7 +47,10 @@ inline bool opt_in(K kernel, OptIn &done, int bytes) {
     if (slot >= 0 && done.bytes[slot].load(std::memory_order_acquire) >= bytes) return true;
     const std::lock_guard<std::mutex> lock(done.growing);
     if ((slot >= 0 ? done.bytes[slot].load(std::memory_order_relaxed) : done.beyond[dev]) >= bytes) return true;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return false;
+    }
     if (slot >= 0)
         done.bytes[slot].store(bytes, std::memory_order_release);
     else
@@ -75,7 +78,8 @@ inline cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, int thread
     config.attrs = attrs;
     config.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
-    return e != cudaSuccess ? e : cudaGetLastError();
+    if (e != cudaSuccess) cudaGetLastError();   // reported by the return value; an earlier call's error is left for its owner
+    return e;
 }
 
 }  // namespace kda

@@ -33,10 +33,25 @@ cudaError_t fake_set_attribute(K, cudaFuncAttribute, int bytes) {
     if (bytes >= 1000) large_set = true;
     return cudaSuccess;
 }
+static cudaError_t pending = cudaSuccess, launch_result = cudaSuccess;   // the runtime's last error, and a launch's own
+static cudaError_t fake_last_error() {
+    const cudaError_t e = pending;
+    pending = cudaSuccess;
+    return e;
+}
+template <typename... P, typename... A>
+cudaError_t fake_launch(const cudaLaunchConfig_t *, void (*)(P...), A &&...) {
+    if (launch_result != cudaSuccess) pending = launch_result;
+    return launch_result;
+}
+#define cudaGetLastError fake_last_error
+#define cudaLaunchKernelEx fake_launch
 #define cudaGetDevice fake_get_device
 #define cudaDeviceGetAttribute fake_get_attribute
 #define cudaFuncSetAttribute fake_set_attribute
 #include "kda_host.cuh"
+#undef cudaGetLastError
+#undef cudaLaunchKernelEx
 #undef cudaGetDevice
 #undef cudaDeviceGetAttribute
 #undef cudaFuncSetAttribute
@@ -92,6 +107,21 @@ def test_devices_beyond_the_table(tmp_path):
         printf("%d %d %d %d %d\n", sms, far, opted, calls.load(), kda::sm_count());
     """)
     assert got == [100, 170, 2000, 2, 100]
+
+
+def test_a_launch_answers_for_itself(tmp_path):
+    """An error that another call left behind is neither this launch's nor taken from whom it is for; a launch that
+    fails reports its own and leaves none behind."""
+    got = run(tmp_path, r"""
+        const auto launch = [] { return kda::launch_overlapped(&kernel, dim3(1), 32, 0, 1, nullptr); };
+        pending = cudaErrorHostMemoryAlreadyRegistered;
+        const int fine = launch(), left = pending;
+        pending = cudaSuccess, launch_result = cudaErrorInvalidValue;
+        const int failed = launch();
+        printf("%d %d %d %d\n", fine == cudaSuccess, left == cudaErrorHostMemoryAlreadyRegistered,
+               failed == cudaErrorInvalidValue, pending == cudaSuccess);
+    """)
+    assert got == [1, 1, 1, 1]
 
 
 RING = r"""
