@@ -12,7 +12,7 @@
 //     output's bytes for short K. A tile of 256 x 256 brings 32 KB to each SM per
 //     128-byte block of K and its 512 cycles of products; two accumulators let the
 //     next tile's products run under the epilogue. 8256 x 12576 x 4096 bf16:
-//     1,300 TFLOP/s at the power limit (the tensor pipe 90% active on 4096 x
+//     1,300 TFLOP/s at the power limit (the tensor pipe 90 to 92% active on 4096 x
 //     9216); 33494 x 4096 x 4096 e4m3 with residual: 2,300 TFLOP/s.
 //   * narrow_kernel, for few tokens, where the weights' bytes are the work:
 //     128 outputs on the lanes x 16..64 tokens as the columns, so that a tile of
