@@ -251,7 +251,7 @@ struct Plan {
     int32_t tiles_t, tiles_n;
     uint32_t idesc, idesc_tail;      // of a whole tile, and of the last one along N (pair_kernel)
     int32_t width, tail;             // their columns: width a multiple of 64, tail of 32
-    int32_t out_tma, residual_tma;   // rows that TMA can store and load
+    int32_t out_tma, residual_tma;   // rows that TMA can store and load (narrow_kernel: that start on 16 bytes)
     int32_t vectors;                 // bias and weight scale start on 16 bytes
 };
 
@@ -330,7 +330,7 @@ __device__ __forceinline__ void box_to_rows(uint8_t *box, O *dst, int64_t stride
 }
 
 // TMA_ROWS: out, and residual where there is one, are rows that TMA stores and
-// loads. The general form holds more registers (3-5% on large products).
+// loads (a store's width a multiple of 16 bytes). The general form holds more registers (3-5% on large products).
 template <typename O, bool E4M3, bool TMA_ROWS>
 __global__ void __launch_bounds__(Pair::kThreads, 1)
     pair_kernel(const KdaLinearArgs p, const Plan plan, const __grid_constant__ Maps maps) {
@@ -1039,7 +1039,9 @@ int launch(const KdaLinearArgs *args, void *workspace, size_t workspace_bytes, c
     const int tile_t = pair ? 256 : c.tile, tile_n = pair ? c.tile : kLanes;
     plan.tiles_t = (a.num_tokens + tile_t - 1) / tile_t;
     plan.tiles_n = (a.out_features + tile_n - 1) / tile_n;
-    plan.out_tma = tma_rows(a.out, a.out_row_stride, a.num_tokens, a.out_features, 2);
+    // A TMA store ends on 16 bytes: past a width that is no multiple of them it would write zeros into what lies
+    // beside the row (a store of 3 columns wrote 8). The narrow kernel stores whole vectors inside the row only.
+    plan.out_tma = tma_rows(a.out, a.out_row_stride, a.num_tokens, a.out_features, 2) && (!pair || a.out_features % 8 == 0);
     plan.residual_tma =
         a.residual != nullptr && tma_rows(a.residual, a.residual_row_stride, a.num_tokens, a.out_features, 2);
     plan.vectors = ((reinterpret_cast<uintptr_t>(a.bias) | reinterpret_cast<uintptr_t>(a.weight_scale)) & 15u) == 0;

@@ -85,6 +85,23 @@ def test_rows_on_and_off_boundaries(types, form, layout):
     assert torch.equal(over, out)
 
 
+@pytest.mark.parametrize("T", [1, 130, 300])
+@pytest.mark.parametrize("N", [1, 3, 14, 65, 177, 260, 515])
+@pytest.mark.parametrize("form", [(PAIR, 64, 1), (PAIR, 128, 1), (PAIR, 192, 1), (PAIR, 256, 1), (NARROW, 16, 2), (NARROW, 64, 1)])
+def test_odd_widths_in_aligned_rows(form, N, T):
+    """Rows that start on 16 bytes and end off them: a column slice of a wider output, whose other columns stay."""
+    K, extra = 128, -N % 8 + 16
+    x, w, s = operands(T, K, N, BF16, N)
+    bias, values = epilogue(T, N, BF16)
+    wide = torch.full((T, 8 + N + extra), 7.0, dtype=BF16, device="cuda")
+    out, residual = wide[:, 8:8 + N], strided(T, N, BF16, 8, extra + 8)
+    residual.copy_(values)
+    for r in (None, residual):
+        wide.fill_(7.0)
+        check(form, x, w, s, out, "silu", bias, r)
+        assert (wide[:, :8] == 7).all() and (wide[:, 8 + N:] == 7).all()
+
+
 @pytest.mark.parametrize("N", [1, 7, 32, 33, 63, 64, 65, 96, 128, 160, 191, 255, 257, 300])
 @pytest.mark.parametrize("width", WIDTHS)
 def test_pair_widths_and_tails(width, N):
